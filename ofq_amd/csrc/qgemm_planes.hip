@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 3
   auto gload = [&](int kt) {
     const int k0 = kt * QBS_BK;
     const bool kina = (k0 + kqa) < K, kinb = (k0 + kqb) < K;       // K % 8 == 0 (host check)
-    rks = *reinterpret_cast<const f32x4v*>(ksp ? ksp + (kina ? k0 + kqa : 0) : A + offA[0]);      // no ksp: any valid address
+    rks = *reinterpret_cast<const f32x4v*>(ksp ? ksp + (kina ? k0 + kqa : 0) : A + offA[0] - kqa);      // no ksp: any valid address
 #pragma unroll
     for (int i = 0; i < 4; ++i) ra[i] = *reinterpret_cast<const f32x4v*>(A + offA[i] + (kina ? k0 : -kqa));
 #pragma unroll
