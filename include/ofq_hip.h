@@ -553,6 +553,42 @@ int ofq_input_pipeline_u8(const uint8_t* in, float* out, int64_t B, int64_t C, i
                           const float* std255, int use_mix, int use_cutmix, float lam, float one_minus_lam, int yl, int yh, int xl,
                           int xh, const int32_t* rects, const float* noise, ofq_stream_t stream);
 
+/* ---- softmax cross entropy of z = x W^T + b over a large vocabulary, from the hidden states on, without keeping the logits
+ *  (csrc/linear_ce.hip): lse_t = log sum_v exp z_tv, loss_t = lse_t - (1 - e) z_t,target - e/V sum_v z_tv with e = smoothing.
+ *  x [T][D], w [V][D] fp32 (bf16 = 0) or bf16 (bf16 = 1), contiguous; bias [V] or NULL, bf16 where bias16; target int64 [T].  Rows
+ *  with target == ignore_index lose nothing and receive no gradient, whatever x holds there; a target outside the vocabulary
+ *  makes its loss NaN.  reduction: 0 none (loss [T]), 1 mean over the live rows (NaN without any), 2 sum; loss and lse [T] fp32.
+ *  kept: what the backward needs beside its arguments (ofq_linear_ce_kept_bytes; w_aligned = w is a multiple of 16 bytes), ws: scratch;
+ *  both 256-byte aligned device memory of the caller.
+ *  bwd: grad = the incoming gradient (one float; reduction 0: [T]); dx [T][D], dw [V][D] in the tensors' type, db [V] in the
+ *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.
+ *  T <= 2^24, V <= 2^24, D <= 2^20. */
+size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned);
+size_t ofq_linear_ce_fwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16);
+size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int want_dx, int want_db);
+int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
+                      int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, float* loss, float* lse,
+                      void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, ofq_stream_t stream);
+int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const int64_t* target, const float* lse, const void* kept,
+                      int64_t T, int64_t D, int64_t V, int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction,
+                      void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream);
+
+/* ---- Newton-Schulz orthogonalisation of many matrices, and the optimiser step around it (csrc/newton_schulz.hip)
+ *  tensors: HOST array of n records of ofq_newton_schulz_entry_bytes() bytes
+ *      { const void* g; float* mom; void* out; int64_t rows, cols; float wscale, reserved; }
+ *  per matrix: U = g, or with a momentum buffer m <- m + (1 - momentum)(g - m) and U = m or (nesterov) m - (1 - momentum)(m - g);
+ *  X = U / max(|U|_F, eps), transposed where rows > cols; steps times A = X X^T, B = b A + c A A, X <- a X + B X.
+ *  Without momentum out <- X in g's type (bf16: all g are bf16, else fp32); with it g is fp32 and the parameter
+ *  out <- out (1 - lr weight_decay) - lr wscale X.  hyper_dev: NULL, or device memory {lr, 1 - lr weight_decay} read instead of the
+ *  arguments (a captured step); guard: NULL or the step-guard word (non-zero: momentum and parameters stay as they are).
+ *  The mom of all records is set, or of none.  ws: 256-byte aligned device scratch of ofq_newton_schulz_ws_bytes (0: bad records).
+ *  The coefficients must keep every |X| element below 60 and |B| below 60 (the planes hold the values times 2^10). */
+int64_t ofq_newton_schulz_entry_bytes(void);
+size_t ofq_newton_schulz_ws_bytes(const void* tensors, int64_t n);
+int ofq_newton_schulz(const void* tensors, int64_t n, int bf16, int steps, float a, float b, float c, float eps, float lr,
+                      float weight_decay, double momentum, int nesterov, const void* hyper_dev, const void* guard, void* ws,
+                      size_t ws_bytes, ofq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

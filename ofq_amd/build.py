@@ -16,7 +16,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "libofq.hip")
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("libofq.hip", "libofq_step.hip")]      # one translation unit each
 OUT_DIR = os.path.join(HERE, "lib")
 OUT = os.path.join(OUT_DIR, "libofq_hip.so")
 ARCH = "gfx950"
@@ -65,17 +65,24 @@ def build(force=False, verbose=False):
                 return OUT
             hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
             tmp = "%s.%d.tmp" % (OUT, os.getpid())
-            cmd = [hipcc, "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared",
-                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-                   '-DOFQ_SOURCE_HASH="%s"' % source_hash(), SRC, "-o", tmp]
+            flags = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC",
+                     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+            objs = ["%s.%d.o" % (tmp, i) for i in range(len(SRCS))]
+            cmds = [[hipcc] + flags + ['-DOFQ_SOURCE_HASH="%s"' % source_hash(), "-c", src, "-o", obj] for src, obj in zip(SRCS, objs)]
+            link = [hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC"] + objs + ["-o", tmp]
             if verbose:
-                print(" ".join(cmd))
+                for cmd in cmds + [link]:
+                    print(" ".join(cmd))
             try:
-                subprocess.check_call(cmd)
+                procs = [subprocess.Popen(cmd) for cmd in cmds]
+                for p, cmd in [(p, cmd) for p, cmd in zip(procs, cmds) if p.wait() != 0]:
+                    raise subprocess.CalledProcessError(p.returncode, cmd)
+                subprocess.check_call(link)
                 os.replace(tmp, OUT)
             finally:
-                if os.path.exists(tmp):
-                    os.remove(tmp)
+                for f in objs + [tmp]:
+                    if os.path.exists(f):
+                        os.remove(f)
             return OUT
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)

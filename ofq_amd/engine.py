@@ -106,11 +106,30 @@ def param_groups_weight_decay(model, weight_decay, skip=()):
     return [{"params": no_decay, "weight_decay": 0.0}, {"params": decay, "weight_decay": weight_decay}]
 
 
-def make_optimizer(model, lr=5.47e-4, weight_decay=0.05, fused=None, hip=None):
+def muon_param_groups(model, weight_decay, skip=()):
+    """Groups for optim.FusedMuon: the weights of the hidden linear layers by the orthogonalised update, everything else (heads, patch
+    embedding, tables, tokens, steps, offsets, norms) by AdamW's rule with timm's no-decay split."""
+    hidden = {id(m.weight) for name, m in model.named_modules()
+              if isinstance(m, torch.nn.Linear) and not name.split(".")[-1].startswith("head")}
+    groups = param_groups_weight_decay(model, weight_decay, skip)
+    matrices = [p for g in groups for p in g["params"] if id(p) in hidden]
+    rest = [dict(g, params=[p for p in g["params"] if id(p) not in hidden], use_muon=False) for g in groups]
+    return [{"params": matrices, "weight_decay": weight_decay}] + rest
+
+
+def make_optimizer(model, lr=5.47e-4, weight_decay=0.05, fused=None, hip=None, opt="adamw"):
     """AdamW with timm's no-decay split.  On a HIP device the multi-tensor kernel of csrc/adamw.hip (ofq_amd.optim.FusedAdamW,
-    same rule / state dict as torch.optim.AdamW, CGA freeze folded in); hip=False selects torch's own fused AdamW."""
-    groups = param_groups_weight_decay(model, weight_decay)
+    same rule / state dict as torch.optim.AdamW, CGA freeze folded in); hip=False selects torch's own fused AdamW.
+    opt="muon": optim.FusedMuon, the hidden layers' weights by the orthogonalised update at AdamW's update size (the same lr)."""
+    if opt not in ("adamw", "muon"):
+        raise ValueError("make_optimizer: opt must be 'adamw' or 'muon' (got %r)" % (opt,))
     on_dev = next(model.parameters()).is_cuda
+    if opt == "muon":
+        if not on_dev or hip is False:
+            raise RuntimeError("make_optimizer: opt='muon' runs on HIP devices only (no CPU fallback)")
+        from .optim import FusedMuon
+        return FusedMuon(muon_param_groups(model, weight_decay), lr=lr, weight_decay=weight_decay, adjust_lr_fn="match_rms_adamw")
+    groups = param_groups_weight_decay(model, weight_decay)
     if hip is None:
         hip = on_dev and os.environ.get("OFQ_TORCH_ADAMW") is None
     if hip:

@@ -1305,3 +1305,66 @@ class AssembleTokensFn(torch.autograd.Function):
         dcls = dpos[:, 0:1]
         ddist = dpos[:, 1:2] if ctx.ntok == 2 else None
         return g[:, ctx.ntok:], dcls, ddist, dpos
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """Cross entropy of x @ weight^T + bias against integer targets, logits never kept (csrc/linear_ce.hip).  The forward leaves the
+    log-sum-exp of every row and the operands' 16-bit planes; the backward recomputes the logits a piece of the vocabulary at a time."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, smoothing, reduction):
+        D = x.shape[-1]
+        red = ops.CE_REDUCTIONS[reduction]
+        x2d, y = x.reshape(-1, D).contiguous(), target.reshape(-1).contiguous()
+        w = weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        with torch.cuda.device(x.device):
+            loss, lse, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red)
+        ctx.save_for_backward(w, b, y, lse, kept)
+        ctx.args = (x.shape, D, ignore_index, smoothing, red, int(x.dtype == torch.bfloat16))
+        return loss.view(target.shape) if red == 0 else loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        w, b, y, lse, kept = ctx.saved_tensors
+        shape, D, ignore_index, smoothing, red, b16 = ctx.args
+        need = ctx.needs_input_grad
+        with torch.cuda.device(w.device):
+            dx, dw, db = ops.linear_ce_bwd(g.reshape(-1).contiguous(), w, b, y, lse, kept, D, ignore_index, smoothing, red, b16,
+                                           want_dx=need[0], want_dw=need[1], want_db=need[2])
+        return dx.view(shape) if dx is not None else None, dw, db, None, None, None, None
+
+
+def linear_cross_entropy(input, weight, target, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """F.cross_entropy(F.linear(input, weight, bias), target, ...) without the logits: input (..., D), weight (V, D), bias (V,),
+    target (...) int64; fp32 or bf16 (input and weight alike; bias fp32 or theirs).  Returns fp32: a scalar, or target's shape for
+    reduction="none".  Rows whose target is ignore_index take no part, whatever input holds there; a target outside 0 .. V-1
+    that is not ignore_index makes the loss NaN.  "mean" is over the rows that take part (NaN if none does)."""
+    if reduction not in ops.CE_REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction must be one of %s (got %r)" % (sorted(ops.CE_REDUCTIONS), reduction))
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("linear_cross_entropy: label_smoothing must be in [0, 1] (got %r)" % (label_smoothing,))
+    if weight.dim() != 2 or input.dim() < 1 or input.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError("linear_cross_entropy: input (..., D) and a non-empty weight (V, D) (got %s, %s)"
+                         % (tuple(input.shape), tuple(weight.shape)))
+    if target.dtype != torch.int64 or target.shape != input.shape[:-1]:
+        raise ValueError("linear_cross_entropy: target must be int64 of shape %s (got %s %s); class probabilities are not supported"
+                         % (tuple(input.shape[:-1]), target.dtype, tuple(target.shape)))
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError("linear_cross_entropy: bias must be (V,) = (%d,) (got %s)" % (weight.shape[0], tuple(bias.shape)))
+    if input.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != input.dtype:
+        raise RuntimeError("ofq_amd: linear_cross_entropy: input and weight must both be float32 or both bfloat16 (got %s, %s)"
+                           % (input.dtype, weight.dtype))
+    if bias is not None and bias.dtype not in (torch.float32, weight.dtype):
+        raise RuntimeError("ofq_amd: linear_cross_entropy: bias must be float32 or %s (got %s)" % (weight.dtype, bias.dtype))
+    for name, t in (("input", input), ("weight", weight), ("target", target), ("bias", bias)):
+        if t is not None and (not t.is_cuda or t.device != input.device):
+            raise RuntimeError("ofq_amd: linear_cross_entropy: %s must live on input's HIP device (got %s, input on %s); there is no "
+                               "CPU fallback" % (name, t.device, input.device))
+    if max(target.numel(), weight.shape[0]) > 1 << 24 or weight.shape[1] > 1 << 20:
+        raise ValueError("linear_cross_entropy: at most 2^24 rows and classes and 2^20 features")
+    if target.numel() == 0:                     # no rows: a sum of nothing (its gradients are zeros), and a mean over nothing
+        total = input.float().sum() + 0.0 * (weight.float().sum() + (0.0 if bias is None else bias.float().sum()))
+        return total.expand(target.shape) if reduction == "none" else total if reduction == "sum" else total * float("nan")
+    return LinearCrossEntropyFn.apply(input, weight, bias, target, int(ignore_index), float(label_smoothing), reduction)

@@ -6,6 +6,7 @@ import math
 import os
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -1412,3 +1413,65 @@ def gemm_bf16x3x3_nt(x2d, planes, bias=None, products=9):
         _chk(lib().ofq_gemm_bf16x3x3_nt(x2d.data_ptr(), planes.data_ptr(), y.data_ptr(), _p(bias), int(products), M, N, K,
                                         x2d.stride(0), planes.stride(1), N, planes.stride(0), _stream()), "ofq_gemm_bf16x3x3_nt")
     return y
+
+
+# ------------------------------------------------------------------------------------------------ linear cross entropy
+CE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _scratch(nbytes, device):
+    """Scratch of one call, from torch's caching allocator: large and of the call's own size, so it is not kept in the per-stream
+    workspace, and a captured graph owns what its launches point at."""
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+
+
+def linear_ce_fwd(x2d, weight, bias, target, ignore_index, smoothing, reduction):
+    """(loss, lse, kept): loss [T] or a scalar, lse [T], both fp32; kept: the operands' planes, for linear_ce_bwd."""
+    T, D = x2d.shape
+    V = weight.shape[0]
+    dev, b16 = x2d.device, int(x2d.dtype == torch.bfloat16)
+    L = lib()
+    kept = _scratch(L.ofq_linear_ce_kept_bytes(T, D, V, b16, int(weight.data_ptr() % 16 == 0)), dev)
+    ws = _scratch(L.ofq_linear_ce_fwd_ws_bytes(T, D, V, b16), dev)
+    loss = torch.empty((T,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    with _Timed("linear cross entropy, forward", 2.0 * T * D * V):
+        _chk(L.ofq_linear_ce_fwd(x2d.data_ptr(), weight.data_ptr(), _p(bias), target.data_ptr(), T, D, V, b16,
+                                 int(bias is not None and bias.dtype == torch.bfloat16), ignore_index, smoothing, reduction,
+                                 loss.data_ptr(), lse.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(), ws.numel(), _stream()),
+             "ofq_linear_ce_fwd")
+    return loss, lse, kept
+
+
+def linear_ce_bwd(grad, weight, bias, target, lse, kept, D, ignore_index, smoothing, reduction, b16, want_dx=True, want_dw=True,
+                  want_db=True):
+    T, V, dev = target.numel(), weight.shape[0], weight.device
+    L = lib()
+    dx = torch.empty((T, D), dtype=weight.dtype, device=dev) if want_dx else None
+    dw = torch.empty_like(weight) if want_dw else None
+    db = torch.empty_like(bias) if want_db and bias is not None else None
+    ws = _scratch(L.ofq_linear_ce_bwd_ws_bytes(T, D, V, b16, int(dx is not None), int(db is not None)), dev)
+    with _Timed("linear cross entropy, backward", 6.0 * T * D * V):
+        _chk(L.ofq_linear_ce_bwd(grad.data_ptr(), weight.data_ptr(), _p(bias), target.data_ptr(), lse.data_ptr(), kept.data_ptr(),
+                                 T, D, V, b16, int(bias is not None and bias.dtype == torch.bfloat16), ignore_index, smoothing,
+                                 reduction, _p(dx), _p(dw), _p(db), ws.data_ptr(), ws.numel(), _stream()),
+             "ofq_linear_ce_bwd")
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------------------------------------ Newton-Schulz
+NS_ENTRY = np.dtype([("g", "i8"), ("mom", "i8"), ("out", "i8"), ("rows", "i8"), ("cols", "i8"), ("wscale", "f4"), ("pad", "f4")])
+
+
+def newton_schulz(table, bf16, steps, coefficients, eps, lr=0.0, weight_decay=0.0, momentum=0.0, nesterov=False, hyper=None,
+                  guard=None, device=None):
+    """table: numpy array of NS_ENTRY records (device pointers inside; see include/ofq_hip.h: ofq_newton_schulz)."""
+    L = lib()
+    assert L.ofq_newton_schulz_entry_bytes() == NS_ENTRY.itemsize
+    nbytes = L.ofq_newton_schulz_ws_bytes(table.ctypes.data, len(table))
+    if nbytes == 0:
+        raise RuntimeError("ofq_amd: newton_schulz: matrices of 1 to 2^20 rows and columns, at most 65536 of them")
+    ws = _scratch(nbytes, device)
+    a, b, c = coefficients
+    _chk(L.ofq_newton_schulz(table.ctypes.data, len(table), int(bf16), steps, a, b, c, eps, lr, weight_decay, momentum, int(nesterov),
+                             hyper, guard, ws.data_ptr(), ws.numel(), _stream()), "ofq_newton_schulz")

@@ -14,7 +14,7 @@ from ..quantizer.lsq import (LsqQuantizer, LsqQuantizerWeight, LsqQuantizer4img,
 from ...deit_vision_transformer import Mlp, to_2tuple
 from ... import ops
 from ...functional import (LinearFn, codes_linear, codes_linear_ok, codes_only_ok, CodeWeightLinearFn,
-                           code_weight_linear_ok)
+                           code_weight_linear_ok, linear_cross_entropy)
 
 
 # Exact integer-code GEMMs (int8 forward, bf16-split dX) instead of the fp32-MFMA GEMM on fake-quant values.
@@ -313,3 +313,11 @@ class LSQ_QLinear4head(nn.Linear):
             raise ValueError("Unknown quant_method")
         xq = self.input_quant_fn.quant(input, self.move_b4.bias, self.move_aft.bias)
         return LinearFn.apply(xq, weight, self.bias)
+
+    def loss(self, input, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+        """cross_entropy(self(input), target) from the quantised operands on, without the logits: for label sets whose logits and
+        their gradient would outweigh the layer (functional.linear_cross_entropy)."""
+        weight = self.lsqw_fn(self.weight)
+        xq = self.input_quant_fn.quant(input, self.move_b4.bias, self.move_aft.bias)
+        return linear_cross_entropy(xq, weight, target, bias=self.bias, ignore_index=ignore_index,
+                                    label_smoothing=label_smoothing, reduction=reduction)

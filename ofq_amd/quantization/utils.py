@@ -38,3 +38,19 @@ class KDLossSoftandHard(nn.Module):
                 return F_ofq.KDLossFn.apply(cls_output, dist_output, soft, hard_target)        # same value, two launches
             return self.KLSoft(dist_output, soft_target) + self.Hard(cls_output, hard_target)
         return self.KLSoft(output, soft_target) + self.Hard(output, hard_target)
+
+
+class LinearCrossEntropy(nn.Module):
+    """The classifier's product and nn.CrossEntropyLoss in one: hidden states, the classifier's weight and bias, integer targets;
+    the logits of a large label set are never kept (functional.linear_cross_entropy).  HIP tensors only."""
+
+    def __init__(self, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+        super().__init__()
+        self.ignore_index, self.label_smoothing, self.reduction = ignore_index, label_smoothing, reduction
+
+    def forward(self, input, weight, target, bias=None):
+        return F_ofq.linear_cross_entropy(input, weight, target, bias=bias, ignore_index=self.ignore_index,
+                                          label_smoothing=self.label_smoothing, reduction=self.reduction)
+
+    def extra_repr(self):
+        return "ignore_index=%d, label_smoothing=%g, reduction=%r" % (self.ignore_index, self.label_smoothing, self.reduction)

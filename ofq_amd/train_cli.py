@@ -33,7 +33,7 @@ def build_parser(cga=False):
     p.add_argument('--epochs', type=int, default=1)
     p.add_argument('--steps-per-epoch', type=int, default=20)
     p.add_argument('--val-steps', type=int, default=2)
-    p.add_argument('--opt', default='adamw')
+    p.add_argument('--opt', default='adamw', help="adamw, or muon: the hidden layers' weights by the orthogonalised update")
     p.add_argument('--lr', type=float, default=5e-4)
     p.add_argument('--min-lr', type=float, default=1e-5)
     p.add_argument('--warmup-lr', type=float, default=1e-6)
@@ -169,8 +169,8 @@ def load_checkpoint(model, path, strict=True, map_location="cpu"):
 def check_supported(args):
     """Flags the reference accepts that this path does not implement must not be dropped silently."""
     bad = []
-    if args.opt.lower() != "adamw":
-        bad.append("--opt %s (only adamw: train_scripts/*, configs/*.yml)" % args.opt)
+    if args.opt.lower() not in ("adamw", "muon"):
+        bad.append("--opt %s (adamw: train_scripts/*, configs/*.yml; or muon)" % args.opt)
     if args.sched != "cosine":
         bad.append("--sched %s (only cosine)" % args.sched)
     if (args.mixup > 0 or args.cutmix > 0) and args.mixup_mode != "batch":
@@ -255,7 +255,8 @@ def main_worker(local_rank, args, cga, spawned):
         for p_ in teacher.parameters():          # the reference leaves them trainable and back-propagates into the teacher
             p_.requires_grad_(False)             # for nothing (no optimizer holds them); the student's gradients are the same
     log(rank, "model: %s, %.2f M parameters" % (args.model, sum(p.numel() for p in model.parameters()) / 1e6))
-    optimizer = engine.make_optimizer(model, lr=args.lr, weight_decay=args.weight_decay)    # train.py:662
+    optimizer = engine.make_optimizer(model, lr=args.lr, weight_decay=args.weight_decay,      # train.py:662
+                                      opt="muon" if args.opt.lower() == "muon" else "adamw")
     start_epoch = 0
     if args.resume:                                                                         # train.py:691-706
         ck = torch.load(args.resume, map_location=dev, weights_only=False)
