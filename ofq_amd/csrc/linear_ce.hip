@@ -17,22 +17,24 @@
 #define CE_PIECE_BYTES (128ll << 20)     // of G: half of the 256 MB last-level cache
 
 struct CeDims {
-  int64_t T, D, V, Tp, Dp, tiles_v, tiles_t;
+  int64_t T, D, V, Tp, Dp, Vp, tiles_v, tiles_t;
   int np;
   bool pack_w;
 };
 static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, CeDims* d) {
   if (T <= 0 || D <= 0 || V <= 0 || T > (1 << 24) || D > (1 << 20) || V > (1 << 24)) return false;
   auto pad = [](int64_t v) { return (v + G16_PAD - 1) / G16_PAD * G16_PAD; };
-  d->T = T; d->D = D; d->V = V; d->Tp = pad(T); d->Dp = pad(D);
-  d->tiles_v = ceil_div(V, G16_T); d->tiles_t = ceil_div(T, G16_T);
+  d->T = T; d->D = D; d->V = V; d->Tp = pad(T); d->Dp = pad(D); d->Vp = pad(V);
+  d->tiles_v = ceil_div(V, 64); d->tiles_t = ceil_div(T, 64);        // at most
   d->np = bf16 ? 1 : 2;
   d->pack_w = !bf16 || d->Dp != D || !w_aligned;
   return true;
 }
 static size_t ce_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// what the forward pass leaves for the backward: [scales][x planes][W planes]
+// what the forward pass leaves for the backward: [scales][x planes][W planes, zero padded to Vp rows; where W is used in place and
+// its last rows do not fill G16_PAD, those, zero padded]
+__host__ __device__ static inline int64_t ce_w_rows(const CeDims& d) { return d.pack_w ? d.Vp : d.Vp != d.V ? G16_PAD : 0; }
 struct CeKept { float* scale; unsigned short* x; unsigned short* w; size_t bytes; };
 static CeKept ce_kept(void* base, const CeDims& d) {
   CeKept k;
@@ -40,7 +42,7 @@ static CeKept ce_kept(void* base, const CeDims& d) {
   size_t at = 0;
   k.scale = (float*)p; at += 256;
   k.x = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * d.Dp * 2);
-  k.w = (unsigned short*)(p + at); if (d.pack_w) at += ce_up((size_t)d.np * d.V * d.Dp * 2);
+  k.w = (unsigned short*)(p + at); at += ce_up((size_t)d.np * ce_w_rows(d) * d.Dp * 2);
   k.bytes = at;
   return k;
 }
@@ -101,15 +103,16 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
     sw = ce_scale(ce_block_max(m, red));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) { k.scale[0] = sx; k.scale[1] = sw; }
-  const int64_t per = d.Dp / 8, rows = d.Tp + (d.pack_w ? d.V : 0), n = rows * per;
+  const int64_t per = d.Dp / 8, rows = d.Tp + ce_w_rows(d), n = rows * per;
+  const int64_t wfirst = d.pack_w ? 0 : d.Vp - G16_PAD;       // the packed rows of W begin here
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t row = i / per;
     const int64_t c = (i - row * per) * 8;
     const bool isx = row < d.Tp;
-    const int64_t t = isx ? row : row - d.Tp;
-    const bool live = isx ? t < d.T && y[t] != ignore : true;
+    const int64_t to = isx ? row : row - d.Tp, t = isx ? to : to + wfirst;
+    const bool live = isx ? t < d.T && y[t] != ignore : t < d.V;
     const int64_t nv = live ? (d.D - c < 8 ? d.D - c : 8) : 0;
-    unsigned short* dst = (isx ? k.x : k.w) + t * d.Dp + c;
+    unsigned short* dst = (isx ? k.x : k.w) + to * d.Dp + c;
     if (NP == 1) {
       const unsigned short* src = reinterpret_cast<const unsigned short*>(isx ? x : w) + t * d.D + c;
       g16_u32x4 v = {0u, 0u, 0u, 0u};
@@ -138,89 +141,109 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
       g16_u32x4 hi, lo;
       g16_split8(v, hi, lo);
       *reinterpret_cast<g16_u32x4*>(dst) = hi;
-      *reinterpret_cast<g16_u32x4*>(dst + (isx ? d.Tp : d.V) * d.Dp) = lo;
+      *reinterpret_cast<g16_u32x4*>(dst + (isx ? d.Tp : d.Vp) * d.Dp) = lo;
     }
   }
+}
+
+// The incoming gradient as the backward launches see it.  reduction mean / sum: one float for all rows; none: one a row, and with two
+// planes the power of two that they share has been taken by ce_weight_kernel.
+struct CeGrad {
+  const float* grad; const float* scale; const float* shared;
+  int reduction;
+};
+__device__ __forceinline__ float ce_uniform(const CeGrad& g) {
+  const float n = g.scale[2];
+  return g.reduction == 1 ? (n > 0.f ? g.grad[0] / n : 0.f) : g.grad[0];
+}
+// what G is multiplied by beside the rows' weights: the power of two that brings the largest into [2^13, 2^14) (|G| <= |w|)
+template <int NP> __device__ __forceinline__ float ce_gscale(const CeGrad& g) {
+  if (NP == 1) return 1.f;
+  return g.reduction ? ce_scale(fabsf(ce_uniform(g))) : g.shared[0];
 }
 
 struct CeLogits {
   G16Op w, x;                  // P, Q
   const void* bias; const int64_t* y; const float* scale;
+  int64_t ignore;
   int bias16, T, Tp, V, Dp, v0, tiles_r, tiles_c;
   float eps;
   float2* part; float* zsum; float* zy;              // forward: [tiles_v][Tp] (max, sum exp), sum of logits; the target's logit
-  const float* lse; const float* wrow; unsigned short* G; int64_t ldg;       // backward
+  const float* lse; CeGrad g; unsigned short* G; int64_t ldg;      // backward
+  float* db;                                         // column sums of G's tiles [tiles_c][ldg], or NULL
 };
 
-template <int NP, bool GRAD>
-__global__ __launch_bounds__(256) void ce_logits_kernel(CeLogits p) {
-  G16_SHARED
-  __shared__ float sbias[G16_T];
-  __shared__ float stat[3][2][G16_T];
+template <int NP, int CFG, bool GRAD, bool DB>
+__global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
+  using C = G16<NP, CFG>;
+  constexpr int TL = C::T;
+  G16_SHARED(NP, CFG)
+  __shared__ float sbias[TL];
+  __shared__ float stat[3][2][TL];
   int tr, tc;
-  g16_tile_of(blockIdx.x, p.tiles_r, p.tiles_c, tr, tc);
-  const int r0 = p.v0 + tr * G16_T, c0 = tc * G16_T;            // the vocabulary is absolute here
+  g16_group(g16_xcd(blockIdx.x, gridDim.x, gridDim.x), p.tiles_r, p.tiles_c, tr, tc);
+  const int r0 = p.v0 + tr * TL, c0 = tc * TL;            // the vocabulary is absolute here
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wid & 1, wc = wid >> 1, lh = lane >> 5;
-  if (tid < G16_T) {
+  if (tid < TL) {
     float b = 0.f;
     if (p.bias && r0 + tid < p.V)
       b = p.bias16 ? g16_f32(reinterpret_cast<const unsigned short*>(p.bias)[r0 + tid]) : reinterpret_cast<const float*>(p.bias)[r0 + tid];
     sbias[tid] = b;
   }
-  g16_f32x16 acc[2][2];
-  g16_tile<NP, false, false>(acc, p.w, p.x, r0, c0, 0, p.Dp, g16_p0, g16_q0, g16_p1, g16_q1);
+  G16Acc<NP, CFG> acc;
+  g16_tile<NP, CFG, false, false>(acc, p.w, p.x, r0, c0, 0, p.Dp, lds);
   const float ix = NP == 2 ? 1.f / p.scale[0] : 1.f, iw = NP == 2 ? 1.f / p.scale[1] : 1.f;       // powers of two: exact
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < C::RB; ++i)
 #pragma unroll
     for (int eb = 0; eb < 4; ++eb) {
-      const float4 b = *reinterpret_cast<const float4*>(sbias + g16_r(wr, i, eb * 4, lane));
+      const float4 b = *reinterpret_cast<const float4*>(sbias + g16_r<CFG>(wr, i, eb * 4, lane));
       const float bb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < C::CB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][eb * 4 + e] = (NP == 2 ? acc[i][j][eb * 4 + e] * ix * iw : acc[i][j][eb * 4 + e]) + bb[e];
     }
   const int nv = p.V - r0;                                      // rows of this tile inside the vocabulary
-  int yl[2];                                                    // the target's row in this tile, or none
+  int yl[C::CB];                                                    // the target's row in this tile, or none
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int c = c0 + g16_c(wc, j, lane);
+  for (int j = 0; j < C::CB; ++j) {
+    const int c = c0 + g16_c<CFG>(wc, j, lane);
     const int64_t y = c < p.T ? p.y[c] : -1;
-    yl[j] = y >= r0 && y < r0 + G16_T && y < p.V ? (int)(y - r0) : -1;
+    yl[j] = y >= r0 && y < r0 + TL && y < p.V ? (int)(y - r0) : -1;
   }
   if constexpr (!GRAD) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < C::CB; ++j) {
       float m = -INFINITY, z = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < C::RB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int r = g16_r(wr, i, e, lane);
+          const int r = g16_r<CFG>(wr, i, e, lane);
           const float v = acc[i][j][e];
           if (r < nv) { m = v > m || v != v ? v : m; z += v; }
-          if (r == yl[j]) p.zy[c0 + g16_c(wc, j, lane)] = v;
+          if (r == yl[j]) p.zy[c0 + g16_c<CFG>(wc, j, lane)] = v;
         }
       const float om = __shfl_xor(m, 32, 64);
       m = om > m || om != om ? om : m;
       const float safe = m == -INFINITY ? 0.f : m;
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < C::RB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += g16_r(wr, i, e, lane) < nv ? __expf(acc[i][j][e] - safe) : 0.f;
+        for (int e = 0; e < 16; ++e) s += g16_r<CFG>(wr, i, e, lane) < nv ? __expf(acc[i][j][e] - safe) : 0.f;
       s += __shfl_xor(s, 32, 64);
       z += __shfl_xor(z, 32, 64);
       if (lh == 0) {
-        const int c = g16_c(wc, j, lane);
+        const int c = g16_c<CFG>(wc, j, lane);
         stat[0][wr][c] = m; stat[1][wr][c] = s; stat[2][wr][c] = z;
       }
     }
     __syncthreads();
-    if (tid < G16_T && c0 + tid < p.T) {
+    if (tid < TL && c0 + tid < p.T) {
       const float m0 = stat[0][0][tid], m1 = stat[0][1][tid];
       const float m = m1 > m0 || m1 != m1 ? m1 : m0;
       const float safe = m == -INFINITY ? 0.f : m;
@@ -230,22 +253,29 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeLogits p) {
       if (p.zsum) p.zsum[at] = stat[2][0][tid] + stat[2][1][tid];
     }
   } else {
-    float w[2], lse[2];
+    float w[C::CB], lse[C::CB];
+    const float uni = p.g.reduction ? ce_uniform(p.g) : 0.f, gs = ce_gscale<NP>(p.g);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int c = c0 + g16_c(wc, j, lane);
-      w[j] = c < p.T ? p.wrow[c] : 0.f;
+    for (int j = 0; j < C::CB; ++j) {
+      const int c = c0 + g16_c<CFG>(wc, j, lane);
+      const int64_t y = c < p.T ? p.y[c] : p.ignore;
+      w[j] = y == p.ignore || y < 0 || y >= p.V ? 0.f : (p.g.reduction ? uni : p.g.grad[c]) * gs;
       lse[j] = c < p.T ? p.lse[c] : 0.f;
     }
+    float colsum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const float ev = p.eps / (float)p.V, on = 1.f - p.eps;
-    g16_store_tile(
+    g16_store_tile<NP, CFG, false>(
         [&](int i, int j, int e) {
-          const int r = g16_r(wr, i, e, lane);
+          const int r = g16_r<CFG>(wr, i, e, lane);
           const float g = (__expf(acc[i][j][e] - lse[j]) - (r == yl[j] ? on : 0.f) - ev) * w[j];
           return r < nv && w[j] != 0.f ? g : 0.f;
         },
         [&](int c, int r, const float (&v)[8]) {
-          const int64_t row = c0 + c, col = tr * G16_T + r;
+          const int64_t row = c0 + c, col = tr * TL + r;
+          if constexpr (DB) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) colsum[e] += v[e];
+          }
           if (row >= p.Tp || col >= p.ldg) return;
           unsigned short* dst = p.G + row * p.ldg + col;
           if constexpr (NP == 1) {
@@ -257,62 +287,45 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeLogits p) {
             *reinterpret_cast<g16_u32x4*>(dst + (int64_t)p.Tp * p.ldg) = lo;
           }
         },
-        g16_p0, g16_q0, g16_p1, g16_q1);
+        [](int, int, const float (&)[8]) {}, lds);
+    if constexpr (DB) {
+      // every thread has eight columns of the rows it stored; the sixteen threads of the same columns meet in LDS
+      constexpr int PER = TL / 8, RR = g16_nt(CFG) / PER;
+      g16_ldsf* red = (g16_ldsf*)lds.p[0];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[(tid / PER) * TL + (tid % PER) * 8 + e] = colsum[e];
+      __syncthreads();
+      if (tid < TL && tr * TL + tid < p.ldg) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < RR; ++k) s += red[k * TL + tid];
+        p.db[(int64_t)tc * p.ldg + tr * TL + tid] = s;
+      }
+    }
   }
 }
 
-// joins the tiles' statistics: 64 tokens to a workgroup, four threads to a token
-__global__ __launch_bounds__(256) void ce_join_kernel(const float2* __restrict__ part, const float* __restrict__ zsum, const float* __restrict__ zy,
-                                                      const int64_t* __restrict__ y, int64_t ignore, int T, int64_t Tp, int V, int tiles,
-                                                      float eps, float* __restrict__ lse, float* __restrict__ rows) {
-  __shared__ float sm[3][4][64];
-  const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
-  const int t = blockIdx.x * 64 + l;
-  float m = -INFINITY, s = 0.f, z = 0.f;
-  if (t < T)
-    for (int k = q; k < tiles; k += 4) {
-      const float2 p = part[(int64_t)k * Tp + t];
-      const float nm = p.x > m || p.x != p.x ? p.x : m;
-      const float safe = nm == -INFINITY ? 0.f : nm;
-      s = s * __expf(m - safe) + p.y * __expf(p.x - safe);
-      m = nm;
-      if (zsum) z += zsum[(int64_t)k * Tp + t];
-    }
-  sm[0][q][l] = m; sm[1][q][l] = s; sm[2][q][l] = z;
-  __syncthreads();
-  if (q != 0 || t >= T) return;
-#pragma unroll
-  for (int k = 1; k < 4; ++k) {
-    const float om = sm[0][k][l];
-    const float nm = om > m || om != om ? om : m;
-    const float safe = nm == -INFINITY ? 0.f : nm;
-    s = s * __expf(m - safe) + sm[1][k][l] * __expf(om - safe);
-    m = nm;
-    z += sm[2][k][l];
-  }
-  const float L = m + logf(s);
-  const int64_t yt = y[t];
-  float loss;
-  if (yt == ignore) loss = 0.f;
-  else if (yt < 0 || yt >= V) loss = NAN;                   // a target outside the vocabulary: loud, but no read out of range
-  else {
-    loss = L - (1.f - eps) * zy[t];
-    if (eps != 0.f) loss -= eps * (z / (float)V);
-  }
-  lse[t] = L;
-  rows[t] = loss;
-}
+// Joins the tiles' statistics, TOK tokens to a workgroup a time and NT / TOK threads to a token; ONE: one workgroup for all of it, and with
+// it the reduction.
+struct CeJoin {
+  const float2* part; const float* zsum; const float* zy; const int64_t* y;
+  int64_t ignore, Tp;
+  int T, V, tiles, reduction;
+  float eps;
+  float* lse; float* rows; float* loss; float* scale;
+};
 
 // number of live rows and, for mean / sum, the loss: one workgroup, a fixed order
-__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ rows, const int64_t* __restrict__ y, int64_t ignore, int T,
-                                                         int reduction, float* __restrict__ loss, float* __restrict__ scale) {
-  __shared__ double rs[16];
-  __shared__ int rn[16];
+template <int NT>
+__device__ __forceinline__ void ce_reduce(const CeJoin& p) {
+  __shared__ double rs[NT / 64];
+  __shared__ int rn[NT / 64];
   double s = 0.0;
   int n = 0;
-  for (int t = threadIdx.x; t < T; t += 1024) {
-    s += rows[t];
-    n += y[t] != ignore;
+  for (int t = threadIdx.x; t < p.T; t += NT) {
+    s += p.rows[t];
+    n += p.y[t] != p.ignore;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -322,48 +335,91 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
   if ((threadIdx.x & 63) == 0) { rs[threadIdx.x >> 6] = s; rn[threadIdx.x >> 6] = n; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) { s += rs[i]; n += rn[i]; }
-    scale[2] = (float)n;
-    if (reduction == 1) *loss = (float)(s / (double)n);      // no live row: 0 / 0, a NaN, as a mean over nothing is
-    else if (reduction == 2) *loss = (float)s;
+    for (int i = 1; i < NT / 64; ++i) { s += rs[i]; n += rn[i]; }
+    p.scale[2] = (float)n;
+    if (p.reduction == 1) *p.loss = (float)(s / (double)n);      // no live row: 0 / 0, a NaN, as a mean over nothing is
+    else if (p.reduction == 2) *p.loss = (float)s;
   }
 }
 
-// w_t = dL/dloss_t (mean: g / live rows; sum: g; none: g_t), zero where the row does not count; two planes: times the power of two that
-// brings the largest into [2^13, 2^14) (|G| <= |w|).  One workgroup; scal[0] = the power's reciprocal
-__global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict__ grad, const int64_t* __restrict__ y, int64_t ignore, int T,
-                                                         int64_t Tp, int V, int reduction, int planes, const float* __restrict__ scale,
-                                                         float* __restrict__ wrow, float* __restrict__ scal) {
-  __shared__ float red[16];
-  const float n = scale[2];
-  const float g0 = reduction ? grad[0] : 0.f;
-  const float f = reduction == 1 ? (n > 0.f ? g0 / n : 0.f) : g0;
-  auto weight = [&](int64_t t) {
-    if (t >= T) return 0.f;
-    const int64_t yt = y[t];
-    if (yt == ignore || yt < 0 || yt >= V) return 0.f;
-    return reduction ? f : grad[t];
-  };
-  float m = 0.f;
-  if (planes == 2) {
-    for (int64_t t = threadIdx.x; t < T; t += 1024) m = fmaxf(m, fabsf(weight(t)));
-    m = ofq_wave_max(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+template <int NT, int TOK, bool ONE>
+__global__ __launch_bounds__(NT) void ce_join_kernel(CeJoin p) {
+  constexpr int PER = NT / TOK;
+  __shared__ float sm[3][PER][TOK];
+  const int l = threadIdx.x % TOK, q = threadIdx.x / TOK;
+  for (int t0 = blockIdx.x * TOK; t0 < p.T; t0 += gridDim.x * TOK) {
+    const int t = t0 + l;
+    float m = -INFINITY, s = 0.f, z = 0.f;
+    if (t < p.T)
+      for (int k = q; k < p.tiles; k += PER) {
+        const float2 v = p.part[(int64_t)k * p.Tp + t];
+        const float nm = v.x > m || v.x != v.x ? v.x : m;
+        const float safe = nm == -INFINITY ? 0.f : nm;
+        s = s * __expf(m - safe) + v.y * __expf(v.x - safe);
+        m = nm;
+        if (p.zsum) z += p.zsum[(int64_t)k * p.Tp + t];
+      }
     __syncthreads();
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, red[i]);
+    sm[0][q][l] = m; sm[1][q][l] = s; sm[2][q][l] = z;
+    for (int half = PER / 2; half > 0; half >>= 1) {
+      __syncthreads();
+      if (q < half) {
+        const float om = sm[0][q + half][l];
+        const float nm = om > m || om != om ? om : m;
+        const float safe = nm == -INFINITY ? 0.f : nm;
+        s = s * __expf(m - safe) + sm[1][q + half][l] * __expf(om - safe);
+        m = nm;
+        z += sm[2][q + half][l];
+        sm[0][q][l] = m; sm[1][q][l] = s; sm[2][q][l] = z;
+      }
+    }
+    if (q == 0 && t < p.T) {
+      const float L = m + logf(s);
+      const int64_t yt = p.y[t];
+      float loss;
+      if (yt == p.ignore) loss = 0.f;
+      else if (yt < 0 || yt >= p.V) loss = NAN;               // a target outside the vocabulary: loud, but no read out of range
+      else {
+        loss = L - (1.f - p.eps) * p.zy[t];
+        if (p.eps != 0.f) loss -= p.eps * (z / (float)p.V);
+      }
+      p.lse[t] = L;
+      p.rows[t] = loss;
+    }
   }
-  const float s = planes == 2 ? ce_scale(m) : 1.f;
-  for (int64_t t = threadIdx.x; t < Tp; t += 1024) wrow[t] = weight(t) * s;
-  if (threadIdx.x == 0) scal[0] = 1.f / s;
+  if constexpr (ONE) {
+    __syncthreads();
+    ce_reduce<NT>(p);
+  }
+}
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(CeJoin p) { ce_reduce<1024>(p); }
+
+// The power of two for rows with gradients of their own, two planes: one workgroup
+__global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict__ grad, const int64_t* __restrict__ y, int64_t ignore, int T,
+                                                         int V, float* __restrict__ shared) {
+  __shared__ float red[16];
+  float m = 0.f;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) {
+    const int64_t yt = y[t];
+    if (yt != ignore && yt >= 0 && yt < V) m = fmaxf(m, fabsf(grad[t]));
+  }
+  m = ofq_wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
+    shared[0] = ce_scale(m);
+  }
 }
 
 struct CeOut {
   G16Op P, Q;
+  const unsigned short* tail;              // dx: P's last G16_PAD rows of k where K ends in front of them, or NULL
   int R, C, K, tiles_r, tiles_c, split;
   float* part; int64_t slot;               // fp32 [split][C][R], accumulated into where acc is set
   int acc;
   void* out; int out16; int64_t ldo;       // else the final tensor, typed, times 1 / (scale * G's scale)
-  const float* scale; const float* scal;
+  const float* scale; CeGrad g;            // scale: of P
 };
 
 // n of eight values (n <= 8) to element `at` of a typed tensor, 16 bytes at a time where aligned
@@ -386,21 +442,28 @@ __device__ __forceinline__ void ce_put(void* out, int out16, int64_t at, int n, 
 }
 
 // dx (QCOL false: P = W [k = v][r = d], Q = G [c = t][k = v]) and dW (QCOL true: P = x [k = t][r = d], Q = G [k = t][c = v])
-template <int NP, bool QCOL>
-__global__ __launch_bounds__(256) void ce_grad_kernel(CeOut p) {
-  G16_SHARED
+template <int NP, int CFG, bool QCOL>
+__global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
+  using C = G16<NP, CFG>;
+  G16_SHARED(NP, CFG)
   int tr, tc;
-  g16_tile_of(blockIdx.x, p.tiles_r, p.tiles_c, tr, tc);
-  constexpr int BK = G16<NP>::BK;
+  g16_group(g16_xcd(blockIdx.x, gridDim.x, gridDim.x), p.tiles_r, p.tiles_c, tr, tc);
+  constexpr int BK = C::BK;
   const int nk = p.K / BK, per = (nk + p.split - 1) / p.split;
   const int kb = min((int)blockIdx.y * per, nk), ke = min(kb + per, nk);
-  g16_f32x16 acc[2][2];
-  g16_tile<NP, true, QCOL>(acc, p.P, p.Q, tr * G16_T, tc * G16_T, kb * BK, ke * BK, g16_p0, g16_q0, g16_p1, g16_q1);
-  const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = p.part ? 1.f : p.scal[0];
-  g16_store_tile([&](int i, int j, int e) { return acc[i][j][e]; },
+  G16Acc<NP, CFG> acc;
+  g16_tile<NP, CFG, true, QCOL>(acc, p.P, p.Q, tr * C::T, tc * C::T, kb * BK, ke * BK, lds);
+  if constexpr (!QCOL) {
+    if (p.tail && blockIdx.y + 1 == p.split) {
+      const G16Op tp = {p.tail, p.P.ld, 0, G16_PAD, p.P.cols}, tq = {p.Q.p + p.K, p.Q.ld, p.Q.plane, p.Q.rows, p.Q.cols};
+      g16_tile<NP, CFG, true, false, true>(acc, tp, tq, tr * C::T, tc * C::T, 0, G16_PAD, lds);
+    }
+  }
+  const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = NP == 2 ? 1.f / ce_gscale<NP>(p.g) : 1.f;
+  g16_store_tile<NP, CFG, false>([&](int i, int j, int e) { return acc[i][j][e]; },
                  [&](int c, int r, const float (&v0)[8]) {
-                   const int64_t row = tc * G16_T + c;
-                   const int col = tr * G16_T + r;
+                   const int64_t row = tc * C::T + c;
+                   const int col = tr * C::T + r;
                    if (row >= p.C || col >= p.R) return;
                    float v[8];
                    if (p.part) {
@@ -418,22 +481,23 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(CeOut p) {
                      ce_put(p.out, p.out16, row * p.ldo + col, p.R - col, v);
                    }
                  },
-                 g16_p0, g16_q0, g16_p1, g16_q1);
+                 [](int, int, const float (&)[8]) {}, lds);
 }
 
 // dx = sum of the split's partials, in order, scaled and typed
-__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, int planes,
-                                                    const float* __restrict__ scale, const float* __restrict__ scal, void* __restrict__ dx,
-                                                    int out16) {
+template <int NP>
+__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, const float* __restrict__ scale,
+                                                    CeGrad g, void* __restrict__ dx, int out16) {
   const int64_t per = d.Dp / 8, n = d.T * per;
-  const float a = planes == 2 ? 1.f / scale[1] : 1.f, b = scal[0];
+  const float a = NP == 2 ? 1.f / scale[0] : 1.f, b = NP == 2 ? 1.f / ce_gscale<NP>(g) : 1.f;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t t = i / per, c = (i - t * per) * 8;
     if (c >= d.D) continue;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float* p = part + t * d.Dp + c;
+#pragma unroll 8
     for (int s = 0; s < split; ++s) {
-      const float* p = part + s * slot + t * d.Dp + c;
-      const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+      const float4 x = *reinterpret_cast<const float4*>(p + s * slot), y = *reinterpret_cast<const float4*>(p + s * slot + 4);
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
 #pragma unroll
@@ -442,43 +506,16 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
   }
 }
 
-// column sums of G over the tokens: partials [gridDim.y][ldg], then the bias gradient
+// the bias gradient from the tiles' column sums, in order
 template <int NP>
-__global__ __launch_bounds__(256) void ce_db_part_kernel(const unsigned short* __restrict__ G, int64_t Tp, int64_t ldg, float* __restrict__ part) {
-  __shared__ float red[8][256];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int64_t col = (blockIdx.x * 32ll + cl) * 8;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (col < ldg)
-    for (int64_t t = blockIdx.y * 8 + rl; t < Tp; t += gridDim.y * 8) {
-      const g16_u32x4 a = *reinterpret_cast<const g16_u32x4*>(G + t * ldg + col);
-      float v[8];
-      if constexpr (NP == 2) {
-        g16_join8(a, *reinterpret_cast<const g16_u32x4*>(G + (Tp + t) * ldg + col), v);
-      } else {
-        const g16_bf16x8 h = __builtin_bit_cast(g16_bf16x8, a);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += v[e];
-    }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) red[rl][cl * 8 + e] = s[e];
-  __syncthreads();
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sum += red[k][threadIdx.x];
-  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
-  if (c < ldg) part[blockIdx.y * ldg + c] = sum;
-}
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int64_t ldg, int ny, int n, const float* __restrict__ scal,
-                                                    void* __restrict__ db, int out16, int64_t at) {
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int64_t ldg, int ny, int n, CeGrad g, void* __restrict__ db,
+                                                    int out16, int64_t at) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= n) return;
   float s = 0.f;
+#pragma unroll 8
   for (int k = 0; k < ny; ++k) s += part[k * ldg + c];
-  s *= scal[0];
+  s *= NP == 2 ? 1.f / ce_gscale<NP>(g) : 1.f;
   if (out16) reinterpret_cast<unsigned short*>(db)[at + c] = g16_bf16(s);
   else reinterpret_cast<float*>(db)[at + c] = s;
 }
@@ -511,9 +548,42 @@ extern "C" size_t ofq_linear_ce_fwd_ws_bytes(int64_t T, int64_t D, int64_t V, in
   return ce_fwd_ws(nullptr, d).bytes;
 }
 
-static G16Op ce_w_op(const CeDims& d, const CeKept& k, const void* w, int64_t v0, bool col) {
+static G16Op ce_w_op(const CeDims& d, const CeKept& k, const void* w, int64_t v0) {
   const unsigned short* p = d.pack_w ? k.w : (const unsigned short*)w;
-  return G16Op{p + (col ? v0 * d.Dp : 0), d.Dp, d.V * d.Dp, (int)(col ? d.V - v0 : d.V), (int)d.Dp};
+  return G16Op{p + v0 * d.Dp, d.Dp, d.Vp * d.Dp, (int)(d.V - v0), (int)d.Dp};
+}
+
+// launches with the tile form of their grid: logits of V' columns (tv: tiles along them), gradient products
+template <bool GRAD>
+static int ce_logits(CeLogits& a, int64_t V, int64_t T, int bf16, int* tv, hipStream_t st) {
+  auto tiles = [&](int t) { return ceil_div(V, t) * ceil_div(T, t); };
+  const int form = g16_form(tiles(64), tiles(128), tiles(256)), t = g16_t(form);
+  a.tiles_r = (int)ceil_div(V, t); a.tiles_c = (int)ceil_div(T, t);
+  if (tv) *tv = a.tiles_r;
+  const dim3 g((unsigned)(a.tiles_r * a.tiles_c));
+#define CE_LOGITS(NP, CFG)                                                                                                    \
+  do {                                                                                                                        \
+    if (GRAD && a.db) hipLaunchKernelGGL((ce_logits_kernel<NP, CFG, GRAD, GRAD>), g, dim3(g16_nt(CFG)), 0, st, a);             \
+    else hipLaunchKernelGGL((ce_logits_kernel<NP, CFG, GRAD, false>), g, dim3(g16_nt(CFG)), 0, st, a);                         \
+  } while (0)
+  if (bf16) { if (form == G16_BIG) CE_LOGITS(1, G16_BIG); else if (form == G16_MID) CE_LOGITS(1, G16_MID); else if (form == G16_DEEP) CE_LOGITS(1, G16_DEEP); else CE_LOGITS(1, G16_TINY); }
+  else { if (form == G16_BIG) CE_LOGITS(2, G16_BIG); else if (form == G16_MID) CE_LOGITS(2, G16_MID); else if (form == G16_DEEP) CE_LOGITS(2, G16_DEEP); else CE_LOGITS(2, G16_TINY); }
+#undef CE_LOGITS
+  OFQ_LAUNCH_CHECK();
+  return 0;
+}
+template <bool QCOL>
+static int ce_grad(CeOut& o, int bf16, hipStream_t st) {
+  auto tiles = [&](int t) { return ceil_div(o.R, t) * ceil_div(o.C, t) * o.split; };
+  const int form = g16_form(tiles(64), tiles(128), tiles(256)), t = g16_t(form);
+  o.tiles_r = (int)ceil_div(o.R, t); o.tiles_c = (int)ceil_div(o.C, t);
+  const dim3 g((unsigned)(o.tiles_r * o.tiles_c), (unsigned)o.split);
+#define CE_GRAD(NP, CFG) hipLaunchKernelGGL((ce_grad_kernel<NP, CFG, QCOL>), g, dim3(g16_nt(CFG)), 0, st, o)
+  if (bf16) { if (form == G16_BIG) CE_GRAD(1, G16_BIG); else if (form == G16_MID) CE_GRAD(1, G16_MID); else if (form == G16_DEEP) CE_GRAD(1, G16_DEEP); else CE_GRAD(1, G16_TINY); }
+  else { if (form == G16_BIG) CE_GRAD(2, G16_BIG); else if (form == G16_MID) CE_GRAD(2, G16_MID); else if (form == G16_DEEP) CE_GRAD(2, G16_DEEP); else CE_GRAD(2, G16_TINY); }
+#undef CE_GRAD
+  OFQ_LAUNCH_CHECK();
+  return 0;
 }
 
 // reduction: 0 none (loss [T]), 1 mean, 2 sum (loss: one float)
@@ -535,50 +605,53 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
                        (const float*)w, V * D, f.amax);
     OFQ_LAUNCH_CHECK();
   }
-  const int64_t chunks = (d.Tp + (d.pack_w ? V : 0)) * (d.Dp / 8);
+  const int64_t chunks = (d.Tp + ce_w_rows(d)) * (d.Dp / 8);
   const dim3 pg((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 4096));
   if (bf16) hipLaunchKernelGGL(ce_pack_kernel<1>, pg, dim3(256), 0, st, x, target, ignore_index, w, d, f.amax, k);
   else hipLaunchKernelGGL(ce_pack_kernel<2>, pg, dim3(256), 0, st, x, target, ignore_index, w, d, f.amax, k);
   OFQ_LAUNCH_CHECK();
   CeLogits a = {};
-  a.w = ce_w_op(d, k, w, 0, false);
+  a.w = ce_w_op(d, k, w, 0);
   a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
-  a.bias = bias; a.bias16 = bias16; a.y = target; a.scale = k.scale;
+  a.bias = bias; a.bias16 = bias16; a.y = target; a.ignore = ignore_index; a.scale = k.scale;
   a.T = (int)T; a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing;
-  a.tiles_r = (int)d.tiles_v; a.tiles_c = (int)d.tiles_t;
   a.part = f.part; a.zsum = smoothing != 0.f ? f.zsum : nullptr; a.zy = f.zy;
-  if (bf16) hipLaunchKernelGGL((ce_logits_kernel<1, false>), dim3((unsigned)tiles), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((ce_logits_kernel<2, false>), dim3((unsigned)tiles), dim3(256), 0, st, a);
-  OFQ_LAUNCH_CHECK();
-  float* rows = reduction == 0 ? loss : f.rows;
-  hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(T, 64)), dim3(256), 0, st, f.part, a.zsum, f.zy, target, ignore_index, (int)T,
-                     d.Tp, (int)V, (int)d.tiles_v, smoothing, lse, rows);
-  OFQ_LAUNCH_CHECK();
-  hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore_index, (int)T, reduction, loss, k.scale);
+  int tv;
+  if (int rc = ce_logits<false>(a, V, T, bf16, &tv, st)) return rc;
+  const CeJoin j = {f.part, a.zsum, f.zy, target, ignore_index, d.Tp, (int)T, (int)V, tv, reduction, smoothing, lse,
+                    reduction == 0 ? loss : f.rows, loss, k.scale};
+  // little to join: one workgroup does that and the sum, one launch less
+  if (T * tv <= 8192) {
+    if (tv <= 64) hipLaunchKernelGGL((ce_join_kernel<1024, 128, true>), dim3(1), dim3(1024), 0, st, j);
+    else hipLaunchKernelGGL((ce_join_kernel<1024, 8, true>), dim3(1), dim3(1024), 0, st, j);
+  } else {
+    hipLaunchKernelGGL((ce_join_kernel<256, 8, false>), dim3((unsigned)std::min<int64_t>(ceil_div(T, 8), 65536)), dim3(256), 0, st, j);
+    OFQ_LAUNCH_CHECK();
+    hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, j);
+  }
   OFQ_LAUNCH_CHECK();
   return 0;
 }
 
-struct CeBwd { int64_t piece, pieces; int split, ny; float* scal; float* wrow; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
+struct CeBwd { int64_t piece, pieces; int split; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
 static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) {
   CeBwd b;
-  const int64_t vp = ceil_div(d.V, G16_T) * G16_T;
-  b.piece = std::min(vp, std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.np) / G16_T * G16_T, G16_T));
+  const int64_t vp = ceil_div(d.V, 128) * 128;
+  b.piece = std::min(vp, std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.np) / 128 * 128, 128));
   b.pieces = ceil_div(vp, b.piece);
-  b.piece = ceil_div(ceil_div(vp, b.pieces), G16_T) * G16_T;             // pieces of one size
+  b.piece = ceil_div(ceil_div(vp, b.pieces), 128) * 128;             // pieces of one size
   b.pieces = ceil_div(vp, b.piece);
   // dx has few tiles and a long k: split it until two workgroups to a CU have work, at no less than eight k-steps each
-  const int64_t tiles = d.tiles_t * ceil_div(d.D, G16_T), steps = b.piece / (d.np == 1 ? 64 : 32);
+  const int64_t tiles = ceil_div(d.T, 128) * ceil_div(d.D, 128), steps = b.piece / (d.np == 1 ? 64 : 32);
   b.split = tiles >= 384 ? 1 : (int)std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 8));
-  b.ny = (int)std::max<int64_t>(1, std::min<int64_t>(d.Tp / 64, 32));
   char* p = (char*)base;
   size_t at = 0;
-  b.scal = (float*)p; at += 256;
-  b.wrow = (float*)(p + at); at += ce_up(d.Tp * 4);
+  b.shared = (float*)p; at += 256;
   b.G = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * b.piece * 2);
   b.slot = d.T * d.Dp;
-  b.part = (float*)(p + at); if (want_dx) at += ce_up((size_t)b.split * b.slot * 4);
-  b.db = (float*)(p + at); if (want_db) at += ce_up((size_t)b.ny * b.piece * 4);
+  b.part = b.split > 1 || b.pieces > 1 ? (float*)(p + at) : nullptr;                    // else dx is written by its product
+  if (want_dx && b.part) at += ce_up((size_t)b.split * b.slot * 4);
+  b.db = (float*)(p + at); if (want_db) at += ce_up((size_t)d.tiles_t * b.piece * 4);
   b.bytes = at;
   return b;
 }
@@ -601,60 +674,51 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
   const CeBwd b = ce_bwd_ws(ws, d, dx != nullptr, db != nullptr);
   if (ws_bytes < b.bytes) return OFQ_ENOWS;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(ce_weight_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore_index, (int)T, d.Tp, (int)V, reduction, d.np, k.scale,
-                     b.wrow, b.scal);
-  OFQ_LAUNCH_CHECK();
+  if (reduction == 0 && d.np == 2) {
+    hipLaunchKernelGGL(ce_weight_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore_index, (int)T, (int)V, b.shared);
+    OFQ_LAUNCH_CHECK();
+  }
+  const CeGrad cg = {grad, k.scale, b.shared, reduction};
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, V - v0);
-    const int64_t np64 = ceil_div(nv, G16_PAD) * G16_PAD;                 // k extent of dx, whole k-steps: G is zero behind the vocabulary
+    const bool tail = !d.pack_w && nv % G16_PAD;                          // (of the last piece: the others are whole tiles)
+    const int64_t kdx = tail ? nv / G16_PAD * G16_PAD : ceil_div(nv, G16_PAD) * G16_PAD;       // G is zero behind the vocabulary
     CeLogits a = {};
-    a.w = ce_w_op(d, k, w, 0, false);
+    a.w = ce_w_op(d, k, w, 0);
     a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
-    a.bias = bias; a.bias16 = bias16; a.y = target; a.scale = k.scale;
+    a.bias = bias; a.bias16 = bias16; a.y = target; a.ignore = ignore_index; a.scale = k.scale;
     a.T = (int)T; a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing; a.v0 = (int)v0;
-    a.tiles_r = (int)ceil_div(nv, G16_T); a.tiles_c = (int)d.tiles_t;
-    a.lse = lse; a.wrow = b.wrow; a.G = b.G; a.ldg = b.piece;
-    const dim3 lg((unsigned)(a.tiles_r * a.tiles_c));
-    if (bf16) hipLaunchKernelGGL((ce_logits_kernel<1, true>), lg, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((ce_logits_kernel<2, true>), lg, dim3(256), 0, st, a);
-    OFQ_LAUNCH_CHECK();
+    a.lse = lse; a.g = cg; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
+    if (int rc = ce_logits<true>(a, nv, T, bf16, nullptr, st)) return rc;
     const int64_t gpl = d.Tp * b.piece;
     if (dw) {
       CeOut o = {};
       o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.R = (int)D; o.C = (int)nv; o.K = (int)d.Tp; o.split = 1;
-      o.tiles_r = (int)ceil_div(D, G16_T); o.tiles_c = (int)ceil_div(nv, G16_T);
-      o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = k.scale; o.scal = b.scal;
-      const dim3 g((unsigned)(o.tiles_r * o.tiles_c));
-      if (bf16) hipLaunchKernelGGL((ce_grad_kernel<1, true>), g, dim3(256), 0, st, o);
-      else hipLaunchKernelGGL((ce_grad_kernel<2, true>), g, dim3(256), 0, st, o);
-      OFQ_LAUNCH_CHECK();
+      o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = k.scale; o.g = cg;
+      if (int rc = ce_grad<true>(o, bf16, st)) return rc;
     }
     if (dx) {
       CeOut o = {};
-      o.P = ce_w_op(d, k, w, v0, true);
+      o.P = ce_w_op(d, k, w, v0);
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
-      o.R = (int)d.Dp; o.C = (int)T; o.K = (int)np64; o.split = b.split;
-      o.tiles_r = (int)ceil_div(d.Dp, G16_T); o.tiles_c = (int)d.tiles_t;
-      o.part = b.part; o.slot = b.slot; o.acc = i > 0; o.scale = k.scale; o.scal = b.scal;
-      const dim3 g((unsigned)(o.tiles_r * o.tiles_c), (unsigned)b.split);
-      if (bf16) hipLaunchKernelGGL((ce_grad_kernel<1, false>), g, dim3(256), 0, st, o);
-      else hipLaunchKernelGGL((ce_grad_kernel<2, false>), g, dim3(256), 0, st, o);
-      OFQ_LAUNCH_CHECK();
+      o.C = (int)T; o.K = (int)kdx; o.split = b.split; o.tail = tail ? k.w : nullptr; o.scale = k.scale + 1; o.g = cg;
+      if (b.part) { o.R = (int)d.Dp; o.part = b.part; o.slot = b.slot; o.acc = i > 0; }
+      else { o.R = (int)D; o.out = dx; o.out16 = bf16; o.ldo = D; }
+      if (int rc = ce_grad<false>(o, bf16, st)) return rc;
     }
     if (db) {
-      const dim3 g((unsigned)ceil_div(b.piece, 256), (unsigned)b.ny);
-      if (bf16) hipLaunchKernelGGL(ce_db_part_kernel<1>, g, dim3(256), 0, st, b.G, d.Tp, b.piece, b.db);
-      else hipLaunchKernelGGL(ce_db_part_kernel<2>, g, dim3(256), 0, st, b.G, d.Tp, b.piece, b.db);
-      OFQ_LAUNCH_CHECK();
-      hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)ceil_div(nv, 256)), dim3(256), 0, st, b.db, b.piece, b.ny, (int)nv, b.scal, db, bias16, v0);
+      const dim3 g((unsigned)ceil_div(nv, 256));
+      if (bf16) hipLaunchKernelGGL(ce_db_kernel<1>, g, dim3(256), 0, st, b.db, b.piece, a.tiles_c, (int)nv, cg, db, bias16, v0);
+      else hipLaunchKernelGGL(ce_db_kernel<2>, g, dim3(256), 0, st, b.db, b.piece, a.tiles_c, (int)nv, cg, db, bias16, v0);
       OFQ_LAUNCH_CHECK();
     }
   }
-  if (dx) {
+  if (dx && b.part) {
     const dim3 g((unsigned)std::min<int64_t>(ceil_div(T * (d.Dp / 8), 256), 8192));
-    hipLaunchKernelGGL(ce_dx_kernel, g, dim3(256), 0, st, b.part, b.slot, b.split, d, d.np, k.scale, b.scal, dx, bf16);
+    if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, cg, dx, bf16);
+    else hipLaunchKernelGGL(ce_dx_kernel<2>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, cg, dx, bf16);
     OFQ_LAUNCH_CHECK();
   }
   return 0;

@@ -25,7 +25,8 @@ struct NsRec {
   int64_t part;            // first partial sum
   int rows, cols, m, n, mp, np;
   float wscale;
-  int e0, s0, x0t, p0;     // prefix sums over the matrices: elementwise blocks, symmetric tiles, X tiles, partials
+  int e0, p0;              // prefix sums over the matrices: elementwise blocks, partials,
+  int s[3], u[3];          // symmetric tiles and X tiles of 64, 128 and 256
   int nparts, per;         // partial sums of this matrix, blocks to each
 };
 
@@ -36,12 +37,12 @@ __global__ void ns_upload_kernel(NsRec* dst, NsUpload u, int n) {
 }
 
 // the matrix that workgroup `id` works on: the last record whose prefix is <= id
-template <int NsRec::*F>
-__device__ __forceinline__ const NsRec& ns_find(const NsRec* t, int n, int id) {
+template <class F>
+__device__ __forceinline__ const NsRec& ns_find(const NsRec* t, int n, int id, F&& first) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t[mid].*F <= id) lo = mid; else hi = mid - 1;
+    if (first(t[mid]) <= id) lo = mid; else hi = mid - 1;
   }
   return t[lo];
 }
@@ -59,7 +60,7 @@ template <bool BF16>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsRec* __restrict__ t, int n, NsStep st, const unsigned* __restrict__ guard,
                                                       double* __restrict__ parts) {
   if (guard != nullptr && (__hip_atomic_load(guard, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & 0x7fffffffu) != 0u) return;
-  const NsRec r = ns_find<&NsRec::p0>(t, n, blockIdx.x);
+  const NsRec r = ns_find(t, n, blockIdx.x, [](const NsRec& r) { return r.p0; });
   const int64_t total = (int64_t)r.rows * r.cols;
   const int64_t chunk = (int64_t)r.per * (NS_BLK * NS_BLK);
   const int64_t first = (int64_t)(blockIdx.x - r.p0) * chunk, end = min(total, first + chunk);
@@ -86,6 +87,19 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsRec* __restrict__ 
     }
     i = end4 + threadIdx.x;
   }
+  if (BF16 && ((uintptr_t)r.g & 15) == 0) {
+    const int64_t end8 = first + ((end - first) & ~(int64_t)7);
+    for (int64_t k = first + threadIdx.x * 8; k < end8; k += 2048) {
+      const g16_u32x4 w = *reinterpret_cast<const g16_u32x4*>(reinterpret_cast<const unsigned short*>(r.g) + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(w[e] << 16), b = __uint_as_float(w[e] & 0xffff0000u);
+        s += (double)a * a;
+        s += (double)b * b;
+      }
+    }
+    i = end8 + threadIdx.x;
+  }
   for (; i < end; i += 256) {
     float u = ns_load<BF16>(r.g, i);
     if (r.mom) {
@@ -109,7 +123,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ 
                                                       const double* __restrict__ parts, _Float16* __restrict__ ws) {
   __shared__ float blk[NS_BLK][NS_BLK + 1];
   __shared__ double red[4];
-  const NsRec r = ns_find<&NsRec::e0>(t, n, blockIdx.x);
+  const NsRec r = ns_find(t, n, blockIdx.x, [](const NsRec& r) { return r.e0; });
   double s = (int)threadIdx.x < r.nparts ? parts[r.part + threadIdx.x] : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -153,23 +167,25 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ 
   }
 }
 
-// A = X X^T (SQUARE false: K = np) or B = b A + c A A (SQUARE true: K = mp): one tile (tr >= tc) of a symmetric matrix
-template <bool SQUARE>
-__global__ __launch_bounds__(256) void ns_sym_kernel(const NsRec* __restrict__ t, int n, float fb, float fc, int odd, _Float16* __restrict__ ws) {
-  G16_SHARED
-  const NsRec& r = ns_find<&NsRec::s0>(t, n, blockIdx.x);
-  const int id = blockIdx.x - r.s0;
-  int tr = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
-  while ((tr + 1) * (tr + 2) / 2 <= id) ++tr;
-  while (tr * (tr + 1) / 2 > id) --tr;
-  const int tc = id - tr * (tr + 1) / 2;
+// One tile (tr >= tc) of a symmetric matrix: A = X X^T (SQUARE false: k along X's rows) or B = b A + c A A (k along A's).
+// Matrices of unlike lengths in one launch of X X^T wait for the longest tiles: cut along k into pieces (added up by the last to
+// arrive) they were no faster, the pieces' way through memory costs what the balance gains.
+template <int CFG, bool SQUARE>
+__global__ __launch_bounds__(g16_nt(CFG)) void ns_sym_kernel(const NsRec* __restrict__ t, int n, float fb, float fc, int odd, int run,
+                                                             _Float16* __restrict__ ws) {
+  using C = G16<2, CFG>;
+  G16_SHARED(2, CFG)
+  const int id = g16_xcd(blockIdx.x, gridDim.x, run);
+  const NsRec& r = ns_find(t, n, id, [](const NsRec& r) { return r.s[C::SIZE]; });
   const int mp = r.mp;
+  int tr, tc;
+  g16_tri(id - r.s[C::SIZE], (mp + C::T - 1) / C::T, tr, tc);
   const int64_t pl = (int64_t)mp * (SQUARE ? mp : r.np);
   const unsigned short* src = reinterpret_cast<const unsigned short*>(ws) + (SQUARE ? r.a : odd ? r.x1 : r.x0);
   const int ld = SQUARE ? mp : r.np;
   const G16Op P = {src, ld, pl, mp, 0};
-  g16_f32x16 acc[2][2];
-  g16_tile<2, false, false>(acc, P, P, tr * G16_T, tc * G16_T, 0, ld, g16_p0, g16_q0, g16_p1, g16_q1);
+  G16Acc<2, CFG> acc;
+  g16_tile<2, CFG, false, false>(acc, P, P, tr * C::T, tc * C::T, 0, ld, lds);
   const int64_t po = (int64_t)mp * mp;
   _Float16* out = ws + (SQUARE ? r.b : r.a);
   const _Float16* in = ws + r.a;
@@ -192,52 +208,43 @@ __global__ __launch_bounds__(256) void ns_sym_kernel(const NsRec* __restrict__ t
     *reinterpret_cast<g16_u32x4*>(out + at) = h;
     *reinterpret_cast<g16_u32x4*>(out + po + at) = l;
   };
-  g16_store_tile(value, [&](int c, int q, const float (&v)[8]) { put(tc * G16_T + c, tr * G16_T + q, v); }, g16_p0, g16_q0, g16_p1, g16_q1);
-  if (tr == tc) return;
-  // the mirrored tile: eight consecutive c of one r, gathered from the tile in LDS (whole since the barrier in g16_store_tile)
-  const float* quarter[4] = {reinterpret_cast<const float*>(g16_p0), reinterpret_cast<const float*>(g16_q0),
-                             reinterpret_cast<const float*>(g16_p1), reinterpret_cast<const float*>(g16_q1)};
-#pragma unroll
-  for (int pass = 0; pass < 8; ++pass) {
-    const int rr = (threadIdx.x & 63) + 64 * (pass & 1), c0 = (threadIdx.x >> 6) * 8;        // c0 within the quarter
-    const float* q = quarter[pass >> 1];
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = q[(c0 + e) * 128 + (((rr >> 2) ^ (c0 + e)) << 2) + (rr & 3)];
-    put(tr * G16_T + rr, tc * G16_T + (pass >> 1) * 32 + c0, v);
-  }
+  auto direct = [&](int c, int q, const float (&v)[8]) { put(tc * C::T + c, tr * C::T + q, v); };
+  auto mirror = [&](int q, int c, const float (&v)[8]) { put(tr * C::T + q, tc * C::T + c, v); };
+  if (tr == tc) g16_store_tile<2, CFG, false>(value, direct, mirror, lds);
+  else g16_store_tile<2, CFG, true>(value, direct, mirror, lds);
 }
 
 // X <- a X + B X: r runs along the columns of X, c along its rows
-__global__ __launch_bounds__(256) void ns_update_kernel(const NsRec* __restrict__ t, int n, float fa, int odd, _Float16* __restrict__ ws) {
-  G16_SHARED
-  const NsRec& r = ns_find<&NsRec::x0t>(t, n, blockIdx.x);
-  const int nr = (r.np + G16_T - 1) / G16_T;
-  const int id = blockIdx.x - r.x0t;
-  const int tc = id / nr, tr = id % nr;
+template <int CFG>
+__global__ __launch_bounds__(g16_nt(CFG)) void ns_update_kernel(const NsRec* __restrict__ t, int n, float fa, int odd, _Float16* __restrict__ ws) {
+  using C = G16<2, CFG>;
+  G16_SHARED(2, CFG)
+  const int id = g16_xcd(blockIdx.x, gridDim.x, CFG == G16_MID ? 64 : 32);
+  const NsRec& r = ns_find(t, n, id, [](const NsRec& r) { return r.u[C::SIZE]; });
   const int mp = r.mp, np = r.np;
+  int tr, tc;
+  g16_group(id - r.u[C::SIZE], (np + C::T - 1) / C::T, (mp + C::T - 1) / C::T, tr, tc);
   const int64_t pl = (int64_t)mp * np;
   const _Float16* x = ws + (odd ? r.x1 : r.x0);
   _Float16* out = ws + (odd ? r.x0 : r.x1);
   const G16Op P = {reinterpret_cast<const unsigned short*>(x), np, pl, mp, np};
   const G16Op Q = {reinterpret_cast<const unsigned short*>(ws) + r.b, mp, (int64_t)mp * mp, mp, 0};
-  g16_f32x16 acc[2][2];
-  g16_tile<2, true, false>(acc, P, Q, tr * G16_T, tc * G16_T, 0, mp, g16_p0, g16_q0, g16_p1, g16_q1);
-  g16_store_tile([&](int i, int j, int e) { return acc[i][j][e] * (1.f / NS_SCALE); },
-                 [&](int c, int q, const float (&v0)[8]) {
-                   const int row = tc * G16_T + c, col = tr * G16_T + q;
-                   if (row >= mp || col >= np) return;
-                   const int64_t at = (int64_t)row * np + col;
-                   float v[8];
-                   g16_join8(*reinterpret_cast<const g16_u32x4*>(x + at), *reinterpret_cast<const g16_u32x4*>(x + pl + at), v);
+  G16Acc<2, CFG> acc;
+  g16_tile<2, CFG, true, false>(acc, P, Q, tr * C::T, tc * C::T, 0, mp, lds);
+  auto put = [&](int c, int q, const float (&v0)[8]) {
+    const int row = tc * C::T + c, col = tr * C::T + q;
+    if (row >= mp || col >= np) return;
+    const int64_t at = (int64_t)row * np + col;
+    float v[8];
+    g16_join8(*reinterpret_cast<const g16_u32x4*>(x + at), *reinterpret_cast<const g16_u32x4*>(x + pl + at), v);
 #pragma unroll
-                   for (int e = 0; e < 8; ++e) v[e] = fa * v[e] + v0[e];
-                   g16_u32x4 h, l;
-                   g16_split8(v, h, l);
-                   *reinterpret_cast<g16_u32x4*>(out + at) = h;
-                   *reinterpret_cast<g16_u32x4*>(out + pl + at) = l;
-                 },
-                 g16_p0, g16_q0, g16_p1, g16_q1);
+    for (int e = 0; e < 8; ++e) v[e] = fa * v[e] + v0[e];
+    g16_u32x4 h, l;
+    g16_split8(v, h, l);
+    *reinterpret_cast<g16_u32x4*>(out + at) = h;
+    *reinterpret_cast<g16_u32x4*>(out + pl + at) = l;
+  };
+  g16_store_tile<2, CFG, false>([&](int i, int j, int e) { return acc[i][j][e] * (1.f / NS_SCALE); }, put, put, lds);
 }
 
 // out = O (the update's own type), or the parameter p <- p decay - lr wscale O; hyper: {lr, decay} from device memory (a captured
@@ -247,7 +254,7 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__
                                                        const unsigned* __restrict__ guard, int odd, const _Float16* __restrict__ ws) {
   if (guard != nullptr && (__hip_atomic_load(guard, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & 0x7fffffffu) != 0u) return;
   __shared__ float blk[NS_BLK][NS_BLK + 1];
-  const NsRec r = ns_find<&NsRec::e0>(t, n, blockIdx.x);
+  const NsRec r = ns_find(t, n, blockIdx.x, [](const NsRec& r) { return r.e0; });
   const float lr = hyper ? hyper[0] : st.lr, decay = hyper ? hyper[1] : st.decay;
   const int bc = r.np / NS_BLK, id = blockIdx.x - r.e0;
   const int xr = (id / bc) * NS_BLK, xc = (id % bc) * NS_BLK;
@@ -289,10 +296,11 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__
 struct NsPlan {
   std::vector<NsRec> recs;
   int64_t halves = 0, parts = 0;
-  int blocks = 0, sym = 0, upd = 0;
+  bool alike = true;       // one length
+  int blocks = 0, sym[3] = {0, 0, 0}, upd[3] = {0, 0, 0};        // tiles of 64, 128 and 256
 };
 
-// the workspace: [records][partial sums][planes]
+// the workspace: [records][partial sums of squares][planes]
 static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
   if (!ts || n <= 0 || n > 65536) return OFQ_EINVAL;
   std::vector<int> order(n);
@@ -305,7 +313,7 @@ static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
     return std::max(ts[x].rows, ts[x].cols) > std::max(ts[y].rows, ts[y].cols);
   });
   auto pad = [](int64_t v) { return (int)((v + G16_PAD - 1) / G16_PAD * G16_PAD); };
-  int64_t blocks = 0, sym = 0, upd = 0;
+  int64_t blocks = 0, sym[3] = {0, 0, 0}, upd[3] = {0, 0, 0};
   for (int64_t k = 0; k < n; ++k) {
     const NsTensor& s = ts[order[k]];
     NsRec r = {};
@@ -323,16 +331,25 @@ static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
     r.p0 = (int)out->parts;
     out->parts += r.nparts;
     r.e0 = (int)blocks; blocks += nb;
-    const int64_t tm = ceil_div(r.mp, G16_T), tn = ceil_div(r.np, G16_T);
-    r.s0 = (int)sym; sym += tm * (tm + 1) / 2;
-    r.x0t = (int)upd; upd += tm * tn;
-    if (blocks >= (1ll << 30) || sym >= (1ll << 24) || upd >= (1ll << 30)) return OFQ_EINVAL;
+    for (int k3 = 0; k3 < 3; ++k3) {
+      const int64_t tm = ceil_div(r.mp, 64 << k3), tn = ceil_div(r.np, 64 << k3);
+      r.s[k3] = (int)sym[k3]; r.u[k3] = (int)upd[k3];
+      sym[k3] += tm * (tm + 1) / 2;
+      upd[k3] += tm * tn;
+    }
+    if (k && r.np != out->recs[0].np) out->alike = false;
+    if (blocks >= (1ll << 30) || sym[0] >= (1ll << 30) || upd[0] >= (1ll << 30)) return OFQ_EINVAL;
     out->recs.push_back(r);
   }
-  out->blocks = (int)blocks; out->sym = (int)sym; out->upd = (int)upd;
+  out->blocks = (int)blocks;
+  for (int k3 = 0; k3 < 3; ++k3) { out->sym[k3] = (int)sym[k3]; out->upd[k3] = (int)upd[k3]; }
   return 0;
 }
 static size_t ns_up(size_t b) { return (b + 255) & ~(size_t)255; }
+
+static size_t ns_bytes(const NsPlan& p) {
+  return ns_up(p.recs.size() * sizeof(NsRec)) + ns_up(p.parts * sizeof(double)) + ns_up(p.halves * 2);
+}
 
 extern "C" int64_t ofq_newton_schulz_entry_bytes(void) { return (int64_t)sizeof(NsTensor); }
 
@@ -340,7 +357,7 @@ extern "C" size_t ofq_newton_schulz_ws_bytes(const void* tensors, int64_t n) {
   try {
     NsPlan p;
     if (ns_plan((const NsTensor*)tensors, n, &p)) return 0;
-    return ns_up(n * sizeof(NsRec)) + ns_up(p.parts * sizeof(double)) + ns_up(p.halves * 2);
+    return ns_bytes(p);
   } catch (...) { return 0; }
 }
 
@@ -356,11 +373,11 @@ extern "C" int ofq_newton_schulz(const void* tensors, int64_t n, int bf16, int s
     for (int64_t i = 0; i < n; ++i) {
       if (!ts[i].g || !ts[i].out || (bf16 && ts[i].mom) || (ts[i].mom != nullptr) != (ts[0].mom != nullptr)) return OFQ_EINVAL;
     }
-    const size_t rb = ns_up(n * sizeof(NsRec)), pb = ns_up(p.parts * sizeof(double));
-    if (!ws || ((uintptr_t)ws & 255) || ws_bytes < rb + pb + ns_up(p.halves * 2)) return OFQ_ENOWS;
-    NsRec* recs = (NsRec*)ws;
-    double* parts = (double*)((char*)ws + rb);
-    _Float16* planes = (_Float16*)((char*)ws + rb + pb);
+    if (!ws || ((uintptr_t)ws & 255) || ws_bytes < ns_bytes(p)) return OFQ_ENOWS;
+    char* at = (char*)ws;
+    NsRec* recs = (NsRec*)at; at += ns_up(n * sizeof(NsRec));
+    double* parts = (double*)at; at += ns_up(p.parts * sizeof(double));
+    _Float16* planes = (_Float16*)at;
     hipStream_t st = (hipStream_t)stream;
     for (int64_t i = 0; i < n; i += NS_UPLOAD) {
       NsUpload u;
@@ -380,13 +397,25 @@ extern "C" int ofq_newton_schulz(const void* tensors, int64_t n, int bf16, int s
     if (bf16) hipLaunchKernelGGL(ns_pack_kernel<true>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, eps, parts, planes);
     else hipLaunchKernelGGL(ns_pack_kernel<false>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, eps, parts, planes);
     OFQ_LAUNCH_CHECK();
+    // unlike lengths: DEEP, in which a long tile alone on a CU is fastest, and short runs (thirty matrices of 384 x 384 and 384 x 1536:
+    // 40 us, MID 50; six of 2048 x 2048 and 2048 x 8192: 390, MID 505, BIG 565)
+    const int cs = g16_form(p.sym[0], p.sym[1], p.sym[2]), ca = p.alike || cs == G16_TINY ? cs : G16_DEEP, cu = g16_form(p.upd[0], p.upd[1], p.upd[2]);
+    auto grid = [](const int (&tiles)[3], int form) { return dim3((unsigned)tiles[form == G16_TINY ? 0 : form == G16_BIG ? 2 : 1]); };
+    const dim3 ga = grid(p.sym, ca), gs = grid(p.sym, cs), gu = grid(p.upd, cu);
+    const int ra = p.alike ? 32 : 4;
     for (int k = 0; k < steps; ++k) {
-      hipLaunchKernelGGL(ns_sym_kernel<false>, dim3(p.sym), dim3(256), 0, st, recs, nn, fb, fc, k & 1, planes);
+#define NS_SYM(CFG, SQ, GRID, RUN) hipLaunchKernelGGL((ns_sym_kernel<CFG, SQ>), GRID, dim3(g16_nt(CFG)), 0, st, recs, nn, fb, fc, k & 1, RUN, planes)
+      if (ca == G16_BIG) NS_SYM(G16_BIG, false, ga, 32); else if (ca == G16_MID) NS_SYM(G16_MID, false, ga, 64);
+      else if (ca == G16_DEEP) NS_SYM(G16_DEEP, false, ga, ra); else NS_SYM(G16_TINY, false, ga, ra);
       OFQ_LAUNCH_CHECK();
-      hipLaunchKernelGGL(ns_sym_kernel<true>, dim3(p.sym), dim3(256), 0, st, recs, nn, fb, fc, k & 1, planes);
+      if (cs == G16_BIG) NS_SYM(G16_BIG, true, gs, 32); else if (cs == G16_MID) NS_SYM(G16_MID, true, gs, 64);
+      else if (cs == G16_DEEP) NS_SYM(G16_DEEP, true, gs, 32); else NS_SYM(G16_TINY, true, gs, 32);
       OFQ_LAUNCH_CHECK();
-      hipLaunchKernelGGL(ns_update_kernel, dim3(p.upd), dim3(256), 0, st, recs, nn, fa, k & 1, planes);
+#undef NS_SYM
+#define NS_UPD(CFG) hipLaunchKernelGGL(ns_update_kernel<CFG>, gu, dim3(g16_nt(CFG)), 0, st, recs, nn, fa, k & 1, planes)
+      if (cu == G16_BIG) NS_UPD(G16_BIG); else if (cu == G16_MID) NS_UPD(G16_MID); else if (cu == G16_DEEP) NS_UPD(G16_DEEP); else NS_UPD(G16_TINY);
       OFQ_LAUNCH_CHECK();
+#undef NS_UPD
     }
     if (bf16) hipLaunchKernelGGL(ns_apply_kernel<true>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, hyper, gd, steps & 1, planes);
     else hipLaunchKernelGGL(ns_apply_kernel<false>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, hyper, gd, steps & 1, planes);

@@ -1318,7 +1318,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         x2d, y = x.reshape(-1, D).contiguous(), target.reshape(-1).contiguous()
         w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        with torch.cuda.device(x.device):
+        with ops.on_device(x.device):
             loss, lse, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red)
         ctx.save_for_backward(w, b, y, lse, kept)
         ctx.args = (x.shape, D, ignore_index, smoothing, red, int(x.dtype == torch.bfloat16))
@@ -1330,7 +1330,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         w, b, y, lse, kept = ctx.saved_tensors
         shape, D, ignore_index, smoothing, red, b16 = ctx.args
         need = ctx.needs_input_grad
-        with torch.cuda.device(w.device):
+        with ops.on_device(w.device):
             dx, dw, db = ops.linear_ce_bwd(g.reshape(-1).contiguous(), w, b, y, lse, kept, D, ignore_index, smoothing, red, b16,
                                            want_dx=need[0], want_dw=need[1], want_db=need[2])
         return dx.view(shape) if dx is not None else None, dw, db, None, None, None, None

@@ -7,6 +7,7 @@ hipGraph: a captured launch keeps its arguments, so inside a capture (engine.Gra
 `_dev` form of the kernel, which reads lr and the bias corrections from device memory, and leaves the step counters
 alone; `advance_for_replay()` -- called before every replay -- advances the counters on the host and stores the new
 scalars (formed by the same host arithmetic as the eager path: bit-identical updates)."""
+import functools
 import math
 
 import numpy as np
@@ -183,27 +184,30 @@ class FusedAdamW(torch.optim.Optimizer):
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def _check_newton_schulz(who, coefficients, steps, eps):
+@functools.lru_cache(maxsize=64)
+def _newton_schulz_in_range(coefficients, steps):
     """The kernels hold X, X X^T and b A + c A A as 16-bit planes of the value times 2^10: coefficients that drive a singular value
     (they all start in [0, 1]) or an eigenvalue of the polynomial past what the planes hold are refused."""
-    if not isinstance(steps, int) or not 0 <= steps <= 100:
-        raise ValueError("%s: the number of steps must be an integer from 0 to 100 (got %r)" % (who, steps))
-    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
-        raise ValueError("%s: three finite coefficients (got %r)" % (who, coefficients))
-    if not eps > 0:
-        raise ValueError("%s: eps must be positive (got %r)" % (who, eps))
     a, b, c = coefficients
     x = np.linspace(0.0, 1.0, 4097)
     with np.errstate(over="ignore", invalid="ignore"):
         for _ in range(steps):
             p = b * x * x + c * x ** 4
             if not (np.abs(p).max() < 32 and (x * x).max() < 32):
-                break
+                return False
             x = a * x + p * x
-        else:
-            if np.abs(x).max() < 32:
-                return
-    raise ValueError("%s: these coefficients let the singular values grow out of range: %r" % (who, tuple(coefficients)))
+    return bool(np.abs(x).max() < 32)
+
+
+def _check_newton_schulz(who, coefficients, steps, eps):
+    if not isinstance(steps, int) or not 0 <= steps <= 100:
+        raise ValueError("%s: the number of steps must be an integer from 0 to 100 (got %r)" % (who, steps))
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
+        raise ValueError("%s: three finite coefficients (got %r)" % (who, coefficients))
+    if not eps > 0:
+        raise ValueError("%s: eps must be positive (got %r)" % (who, eps))
+    if not _newton_schulz_in_range(tuple(float(c) for c in coefficients), steps):
+        raise ValueError("%s: these coefficients let the singular values grow out of range: %r" % (who, tuple(coefficients)))
 
 
 @torch.no_grad()
@@ -226,10 +230,8 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
         if g.numel():
             runs.setdefault((g.device, g.dtype), []).append((g.contiguous(), o))
     for (dev, dtype), pairs in runs.items():
-        table = np.zeros(len(pairs), dtype=ops.NS_ENTRY)
-        for i, (g, o) in enumerate(pairs):
-            table[i] = (g.data_ptr(), 0, o.data_ptr(), g.shape[0], g.shape[1], 1.0, 0.0)
-        with torch.cuda.device(dev):
+        table = np.array([(g.data_ptr(), 0, o.data_ptr(), g.shape[0], g.shape[1], 1.0, 0.0) for g, o in pairs], dtype=ops.NS_ENTRY)
+        with ops.on_device(dev):
             ops.newton_schulz(table, dtype == torch.bfloat16, steps, coefficients, eps, device=dev)
     return outs[0] if single else outs
 
@@ -279,8 +281,8 @@ class FusedMuon(FusedAdamW):
         super().set_frozen(param, mask)
 
     @staticmethod
-    def _lr_scale(group, p):
-        r, c = p.shape
+    def _lr_scale(group, shape):
+        r, c = shape
         return 0.2 * math.sqrt(max(r, c)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, r / c))
 
     def _advance_class(self, gc):
@@ -294,32 +296,35 @@ class FusedMuon(FusedAdamW):
     def _step_group(self, group, capturing):
         if not group["use_muon"]:
             return super()._step_group(_AdamWView(group), capturing)
-        runs = {}
+        runs, scales, state, f32 = {}, {}, self.state, torch.float32
         for p in group["params"]:
-            if p.grad is None or p.numel() == 0:
+            g = p.grad
+            if g is None or p.numel() == 0:
                 continue
-            if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous() or p.grad.dtype != torch.float32 \
-                    or not p.grad.is_contiguous() or p.grad.device != p.device:
+            dev = p.device
+            if dev.type != "cuda" or p.dtype != f32 or not p.is_contiguous() or g.dtype != f32 or not g.is_contiguous() or g.device != dev:
                 raise RuntimeError("FusedMuon: contiguous fp32 parameters and gradients on a HIP device only (no CPU fallback)")
-            st = self.state[p]
-            if "momentum_buffer" not in st:
+            shape = p.shape
+            buf = state[p].get("momentum_buffer")
+            if buf is None:
                 if capturing:
                     raise RuntimeError("FusedMuon: optimizer state must exist before a capture (a buffer allocated inside a capture "
                                        "would be re-zeroed by every replay); run an eager step first")
-                st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-            buf = st["momentum_buffer"]
-            if buf.dtype != torch.float32 or buf.shape != p.shape or not buf.is_contiguous() or buf.device != p.device:
+                buf = state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            elif buf.dtype != f32 or buf.shape != shape or not buf.is_contiguous() or buf.device != dev:
                 raise RuntimeError("FusedMuon: momentum_buffer must be a contiguous fp32 tensor of its parameter's shape and device")
-            runs.setdefault(p.device, []).append(p)
-        for dev, ps in runs.items():
-            table = np.zeros(len(ps), dtype=ops.NS_ENTRY)
-            for i, p in enumerate(ps):
-                table[i] = (p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr(), p.data_ptr(), p.shape[0], p.shape[1],
-                            self._lr_scale(group, p), 0.0)
-            hyper = self._captured_hyper(group, ps).data_ptr() if capturing else None
-            with torch.cuda.device(dev):
-                ops.newton_schulz(table, False, group["ns_steps"], group["ns_coefficients"], group["eps"], float(group["lr"]),
-                                  float(group["weight_decay"]), float(group["momentum"]), group["nesterov"], hyper,
+            scale = scales.get(shape)
+            if scale is None:
+                scale = scales[shape] = self._lr_scale(group, shape)
+            rows = runs.get(dev)
+            if rows is None:
+                rows = runs[dev] = []
+            rows.append((g.data_ptr(), buf.data_ptr(), p.data_ptr(), shape[0], shape[1], scale, 0.0))
+        for dev, rows in runs.items():
+            hyper = self._captured_hyper(group, None).data_ptr() if capturing else None
+            with ops.on_device(dev):
+                ops.newton_schulz(np.array(rows, dtype=ops.NS_ENTRY), False, group["ns_steps"], group["ns_coefficients"], group["eps"],
+                                  float(group["lr"]), float(group["weight_decay"]), float(group["momentum"]), group["nesterov"], hyper,
                                   ops.step_guard_ptr(dev) or None, device=dev)
 
 
