@@ -553,25 +553,24 @@ int ofq_input_pipeline_u8(const uint8_t* in, float* out, int64_t B, int64_t C, i
                           const float* std255, int use_mix, int use_cutmix, float lam, float one_minus_lam, int yl, int yh, int xl,
                           int xh, const int32_t* rects, const float* noise, ofq_stream_t stream);
 
-/* ---- softmax cross entropy of z = x W^T + b over a large vocabulary, from the hidden states on, without keeping the logits
+/* ---- softmax cross entropy of z = x W^T + b over a large vocabulary, from the hidden states on; logits beyond 128 MB are not kept
  *  (csrc/linear_ce.hip): lse_t = log sum_v exp z_tv, loss_t = lse_t - (1 - e) z_t,target - e/V sum_v z_tv with e = smoothing.
  *  x [T][D], w [V][D] fp32 (bf16 = 0) or bf16 (bf16 = 1), contiguous; bias [V] or NULL, bf16 where bias16; target int64 [T].  Rows
- *  with target == ignore_index lose nothing and receive no gradient, whatever x holds there; a target outside the vocabulary
- *  makes its loss NaN.  reduction: 0 none (loss [T]), 1 mean over the live rows (NaN without any), 2 sum; loss and lse [T] fp32.
- *  kept: what the backward needs beside its arguments (ofq_linear_ce_kept_bytes; w_aligned = w is a multiple of 16 bytes), ws: scratch;
- *  both 256-byte aligned device memory of the caller.
+ *  with target == ignore_index lose nothing, receive no gradient, whatever x holds there, and cost nothing; a target outside the
+ *  vocabulary makes its loss NaN.  reduction: 0 none (loss [T]), 1 mean over the other rows (NaN without any), 2 sum; loss fp32.
+ *  kept: what the backward needs beside its arguments (ofq_linear_ce_kept_bytes; w_aligned = w is a multiple of 16 bytes; backward = 0:
+ *  none is to come), ws: scratch; both 256-byte aligned device memory of the caller.
  *  bwd: grad = the incoming gradient (one float; reduction 0: [T]); dx [T][D], dw [V][D] in the tensors' type, db [V] in the
  *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.
  *  T <= 2^24, V <= 2^24, D <= 2^20. */
-size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned);
+size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, int backward);
 size_t ofq_linear_ce_fwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16);
 size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int want_dx, int want_db);
 int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
-                      int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, float* loss, float* lse,
+                      int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, int backward, float* loss,
                       void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, ofq_stream_t stream);
-int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const int64_t* target, const float* lse, const void* kept,
-                      int64_t T, int64_t D, int64_t V, int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction,
-                      void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream);
+int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, int64_t T, int64_t D, int64_t V,
+                      int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream);
 
 /* ---- Newton-Schulz orthogonalisation of many matrices, and the optimiser step around it (csrc/newton_schulz.hip)
  *  tensors: HOST array of n records of ofq_newton_schulz_entry_bytes() bytes

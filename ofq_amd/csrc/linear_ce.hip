@@ -1,15 +1,16 @@
 // Softmax cross entropy of z = x W^T + b over a large vocabulary, from the hidden states on, without keeping the logits.
-//   forward   lse_t = log sum_v exp z_tv, in one pass over the vocabulary: every 128 x 128 tile of logits leaves (max, sum of
+//   forward   lse_t = log sum_v exp z_tv, in one pass over the vocabulary: every tile of logits leaves (max, sum of
 //             exp) per token, a second launch joins them;  loss_t = lse_t - (1 - e) z_t,y - e/V sum_v z_tv
 //   backward  in pieces of the vocabulary: G = w_t (exp(z - lse_t) - (1 - e)[v = y_t] - e/V) for one piece, recomputed, in 16-bit
 //             planes; dx += G W and dW = G^T x of that piece; db = column sums of G
 // The tile computes z transposed (r = vocabulary, c = token): a lane holds 32 logits of one token, so the softmax statistics
 // need one exchange between lane halves instead of five steps for each of 32 rows.
-// bf16 tensors go to the matrix cores as they are, G is rounded to bf16 (2^-9 relative, unbiased, T V of them to a sum: below the
-// rounding of the bf16 gradients themselves).  fp32 tensors are split into two fp16 planes scaled by a power of two taken from the
+// bf16 tensors go to the matrix cores as they are, G is rounded to bf16 (2^-9 relative, as the gradients themselves are; what all its
+// rows have in common is left out of it, CeGrad).  fp32 tensors are split into two fp16 planes scaled by a power of two taken from the
 // tensor's largest element (gemm16.h); G likewise.  Statistics, sums and partial gradients are fp32.
-// Rows whose target is ignore_index are packed as zeros and weighted zero: whatever they hold (NaN, Inf) reaches nothing.
-// Bound by the matrix cores: 8 T V D operations, of which the recomputation is 2 T V D; for few tokens by the reading of W.
+// Rows whose target is ignore_index are left out of all of it (CeRows): they cost nothing and what they hold (NaN, Inf) reaches nothing.
+// Bound by the matrix cores: 8 n V D operations for n rows that count, of which the recomputation is 2 n V D (6 where the logits are kept,
+// ce_z); for few rows by the reading of W.
 #include "gemm16.h"
 
 #define CE_AMAX_X 128                    // partial maxima of x and of W
@@ -32,21 +33,55 @@ static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, Ce
 }
 static size_t ce_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// what the forward pass leaves for the backward: [scales][x planes][W planes, zero padded to Vp rows; where W is used in place and
-// its last rows do not fill G16_PAD, those, zero padded]
+// Pieces of the vocabulary in the backward pass, and the columns of one: all of it, or as many as give whole rounds of 256 tiles to the 256
+// CUs in dW (and, for as many rows, in G), the last one what is left.  100000 columns of 4096, 4096 rows: seven of 14336 are 3.5 rounds
+// each, 12.9 ms; six of 16384 and a rest 12.0.
+static int64_t ce_pieces(const CeDims& d, int64_t* piece) {
+  const int64_t vp = ceil_div(d.V, 128) * 128, most = std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.np) / 128 * 128, 128);
+  const int64_t round = std::max<int64_t>(256 / ceil_div(d.D, 256), 1) * 256;
+  *piece = vp <= most ? vp : most >= round ? most / round * round : most;
+  return ceil_div(vp, *piece);
+}
+static int ce_form(int64_t R, int64_t C, int split) {
+  auto tiles = [&](int t) { return ceil_div(R, t) * ceil_div(C, t) * split; };
+  return g16_form(tiles(64), tiles(128), tiles(256));
+}
+// Logits of a single piece are kept (its G takes as much again for a while) where the product takes longer than their way to memory and
+// back; else they are computed a second time.  Kept / not, us, 2 directions: bf16, 64 x 65536, D 2048: 267 / 306; 509 x 21841, D 768:
+// 160 / 168; 1024 x 16000, D 256: 112 / 104; fp32, D 768: 331 / 385; 1024 x 16000, D 256: 190 / 195; 700 x 20000, D 64: 123 / 115.
+// Whole tiles, as they lie in the registers; 0: not kept.
+static int64_t ce_z(const CeDims& d) {
+  int64_t piece;
+  if (ce_pieces(d, &piece) > 1 || d.Dp * (d.np == 2 ? 3 : 1) < 512) return 0;
+  const int t = g16_t(ce_form(d.V, d.T, 1));
+  const int64_t n = ceil_div(d.V, t) * ceil_div(d.T, t) * t * t;
+  return n * 4 <= CE_PIECE_BYTES ? n : 0;
+}
+
+// What the forward pass leaves for the backward.  Rows whose target is ignore_index take no part in anything: the others are packed in
+// their order, n of them.  W planes: zero padded to Vp rows; where W is used in place and its last rows do not fill G16_PAD, those, zero
+// padded.
+struct CeRows { int* n; int* pos; int* idx; int* y; float* lse; };    // [1]; row -> packed row or -1; packed -> row; target or -1; lse
 __host__ __device__ static inline int64_t ce_w_rows(const CeDims& d) { return d.pack_w ? d.Vp : d.Vp != d.V ? G16_PAD : 0; }
-struct CeKept { float* scale; unsigned short* x; unsigned short* w; size_t bytes; };
-static CeKept ce_kept(void* base, const CeDims& d) {
+struct CeKept { float* scale; CeRows rows; unsigned short* x; unsigned short* w; float* z; size_t bytes; };
+static CeKept ce_kept(void* base, const CeDims& d, bool backward) {
   CeKept k;
   char* p = (char*)base;
   size_t at = 0;
-  k.scale = (float*)p; at += 256;
+  k.scale = (float*)p; k.rows.n = (int*)p + 2; at += 256;            // scale: 2^Ex, 2^Ew
+  k.rows.pos = (int*)(p + at); at += ce_up(d.Tp * 4);
+  k.rows.idx = (int*)(p + at); at += ce_up(d.Tp * 4);
+  k.rows.y = (int*)(p + at); at += ce_up(d.Tp * 4);
+  k.rows.lse = (float*)(p + at); at += ce_up(d.Tp * 4);
   k.x = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * d.Dp * 2);
   k.w = (unsigned short*)(p + at); at += ce_up((size_t)d.np * ce_w_rows(d) * d.Dp * 2);
+  const int64_t z = backward ? ce_z(d) : 0;
+  k.z = z ? (float*)(p + at) : nullptr; at += ce_up((size_t)z * 4);
   k.bytes = at;
   return k;
 }
-// scale: [0] 2^Ex, [1] 2^Ew, [2] number of live rows
+// packed rows that are zero filled and multiplied
+__device__ __forceinline__ int ce_padded(int n) { return max((n + G16_PAD - 1) / G16_PAD * G16_PAD, G16_PAD); }
 
 __device__ __forceinline__ float ce_block_max(float m, float* red) {
   m = ofq_wave_max(m);
@@ -66,10 +101,64 @@ __device__ __forceinline__ float ce_scale(float m) {
   return __uint_as_float((unsigned)(e + 127) << 23);
 }
 
+// Numbers the rows that count, in order; one workgroup, eight times 64 rows to a wave a time.  rows_out: losses of reduction none, zero for
+// the others (else NULL)
+template <int NT>
+__device__ __forceinline__ void ce_number(const int64_t* __restrict__ y, int64_t ignore, int64_t T, int V, CeRows k, float* __restrict__ rows_out) {
+  __shared__ int count[NT / 64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  int first = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += NT * 8) {
+    const int64_t at = t0 + wid * 512 + lane;
+    int64_t v[8];
+    int before[8], n = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = at + u * 64 < T ? y[at + u * 64] : ignore;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const unsigned long long live = __ballot(v[u] != ignore);
+      before[u] = n + __popcll(live & ((1ull << lane) - 1));
+      n += __popcll(live);
+    }
+    __syncthreads();
+    if (lane == 0) count[wid] = n;
+    __syncthreads();
+    int base = first;
+    for (int w = 0; w < NT / 64; ++w) {
+      if (w < wid) base += count[w];
+      first += count[w];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t t = at + u * 64;
+      if (t >= T) continue;
+      const bool live = v[u] != ignore;
+      const int c = base + before[u];
+      k.pos[t] = live ? c : -1;
+      if (live) {
+        k.idx[c] = (int)t;
+        k.y[c] = v[u] < 0 || v[u] >= V ? -1 : (int)v[u];
+      } else if (rows_out) {
+        rows_out[t] = 0.f;
+      }
+    }
+  }
+  if (threadIdx.x == 0) *k.n = first;
+}
+__global__ __launch_bounds__(1024) void ce_number_kernel(const int64_t* __restrict__ y, int64_t ignore, int64_t T, int V, CeRows k,
+                                                         float* __restrict__ rows_out) {
+  ce_number<1024>(y, ignore, T, V, k, rows_out);
+}
+
 __global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ x, const int64_t* __restrict__ y, int64_t ignore, int64_t T,
-                                                      int64_t D, const float* __restrict__ w, int64_t nw, float* __restrict__ parts) {
+                                                      int64_t D, int V, const float* __restrict__ w, int64_t nw, float* __restrict__ parts,
+                                                      CeRows k, float* __restrict__ rows_out) {
   __shared__ float red[4];
   float m = 0.f;
+  if (blockIdx.x == CE_AMAX_X + CE_AMAX_W) {
+    ce_number<256>(y, ignore, T, V, k, rows_out);
+    return;
+  }
   if (blockIdx.x < CE_AMAX_X) {
     for (int64_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < T; t += CE_AMAX_X * 4) {
       if (y[t] == ignore) continue;
@@ -88,11 +177,11 @@ __global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) parts[blockIdx.x] = m;
 }
 
-// x (rows with ignored targets as zeros, padding as zeros) and, where it cannot be used in place, W into planes; one thread to
-// eight elements of a row
+// x (the rows that count, and zeros up to ce_padded of them) and, where it cannot be used in place, W into planes; one thread to eight
+// elements of a row
 template <int NP>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x, const int64_t* __restrict__ y, int64_t ignore,
-                                                      const void* __restrict__ w, CeDims d, const float* __restrict__ parts, CeKept k) {
+__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x, const void* __restrict__ w, CeDims d, const float* __restrict__ parts,
+                                                      CeKept k) {
   __shared__ float red[4];
   float sx = 1.f, sw = 1.f;
   if (NP == 2) {
@@ -103,14 +192,16 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
     sw = ce_scale(ce_block_max(m, red));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) { k.scale[0] = sx; k.scale[1] = sw; }
-  const int64_t per = d.Dp / 8, rows = d.Tp + ce_w_rows(d), n = rows * per;
+  const int live_rows = *k.rows.n, padded = ce_padded(live_rows);
+  const int64_t per = d.Dp / 8, rows = padded + ce_w_rows(d), n = rows * per;
   const int64_t wfirst = d.pack_w ? 0 : d.Vp - G16_PAD;       // the packed rows of W begin here
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t row = i / per;
     const int64_t c = (i - row * per) * 8;
-    const bool isx = row < d.Tp;
-    const int64_t to = isx ? row : row - d.Tp, t = isx ? to : to + wfirst;
-    const bool live = isx ? t < d.T && y[t] != ignore : t < d.V;
+    const bool isx = row < padded;
+    const int64_t to = isx ? row : row - padded;
+    const bool live = isx ? to < live_rows : to + wfirst < d.V;
+    const int64_t t = !live ? 0 : isx ? k.rows.idx[to] : to + wfirst;
     const int64_t nv = live ? (d.D - c < 8 ? d.D - c : 8) : 0;
     unsigned short* dst = (isx ? k.x : k.w) + to * d.Dp + c;
     if (NP == 1) {
@@ -146,30 +237,36 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
   }
 }
 
-// The incoming gradient as the backward launches see it.  reduction mean / sum: one float for all rows; none: one a row, and with two
-// planes the power of two that they share has been taken by ce_weight_kernel.
+// The incoming gradient as the backward launches see it.  reduction mean / sum: one float for all rows; none: one a row, their largest in
+// shared[0].  G holds (exp(z - lse) - (1 - e)[v = y] - e/V) / unit, times a row's share of the largest gradient: what all rows have in
+// common is multiplied in fp32 at the end.  A target's element, the one that carries a gradient, is then -1 for a class that is not
+// learnt yet, which 16 bits hold exactly; 1/n or 1 - e rounded to bf16 would be one relative error, up to 2^-9, common to all rows, that
+// no sum averages (dW and dx of 7373 rows of bf16: 2.8e-3 from the formula's in 64 bits, against 2.0e-3 so).
 struct CeGrad {
-  const float* grad; const float* scale; const float* shared;
+  const float* grad; const int* n; const float* shared;
   int reduction;
+  float eps;
 };
-__device__ __forceinline__ float ce_uniform(const CeGrad& g) {
-  const float n = g.scale[2];
-  return g.reduction == 1 ? (n > 0.f ? g.grad[0] / n : 0.f) : g.grad[0];
+__device__ __forceinline__ float ce_unit(float eps) { return eps <= 0.5f ? 1.f - eps : 1.f; }
+// two planes: |G| <= 2^14, as the scaled operands are
+template <int NP> __device__ __forceinline__ constexpr float ce_gscale() { return NP == 2 ? 8192.f : 1.f; }
+template <int NP> __device__ __forceinline__ float ce_factor(const CeGrad& g) {
+  const float n = (float)*g.n;
+  const float common = g.reduction == 0 ? g.shared[0] : g.reduction == 2 ? g.grad[0] : n > 0.f ? g.grad[0] / n : 0.f;
+  return common * ce_unit(g.eps) * (1.f / ce_gscale<NP>());
 }
-// what G is multiplied by beside the rows' weights: the power of two that brings the largest into [2^13, 2^14) (|G| <= |w|)
-template <int NP> __device__ __forceinline__ float ce_gscale(const CeGrad& g) {
-  if (NP == 1) return 1.f;
-  return g.reduction ? ce_scale(fabsf(ce_uniform(g))) : g.shared[0];
-}
+// a sum of nothing stays zero under an infinite gradient: rows that are ignored, classes behind a mask
+__device__ __forceinline__ float ce_times(float v, float f) { return v == 0.f ? 0.f : v * f; }
 
 struct CeLogits {
   G16Op w, x;                  // P, Q
-  const void* bias; const int64_t* y; const float* scale;
-  int64_t ignore;
-  int bias16, T, Tp, V, Dp, v0, tiles_r, tiles_c;
+  CeRows rows;
+  const void* bias; const float* scale;
+  float* z;                                          // tiles of logits as they lie in the registers, or NULL
+  int bias16, Tp, V, Dp, v0, tiles_r, tiles_c;
   float eps;
   float2* part; float* zsum; float* zy;              // forward: [tiles_v][Tp] (max, sum exp), sum of logits; the target's logit
-  const float* lse; CeGrad g; unsigned short* G; int64_t ldg;      // backward
+  CeGrad g; unsigned short* G; int64_t ldg;          // backward
   float* db;                                         // column sums of G's tiles [tiles_c][ldg], or NULL
 };
 
@@ -183,69 +280,125 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
   int tr, tc;
   g16_group(g16_xcd(blockIdx.x, gridDim.x, gridDim.x), p.tiles_r, p.tiles_c, tr, tc);
   const int r0 = p.v0 + tr * TL, c0 = tc * TL;            // the vocabulary is absolute here
+  const int n = *p.rows.n;
+  if (c0 >= ce_padded(n)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wid & 1, wc = wid >> 1, lh = lane >> 5;
-  if (tid < TL) {
+  if (p.bias && tid < TL) {
     float b = 0.f;
-    if (p.bias && r0 + tid < p.V)
+    if (r0 + tid < p.V)
       b = p.bias16 ? g16_f32(reinterpret_cast<const unsigned short*>(p.bias)[r0 + tid]) : reinterpret_cast<const float*>(p.bias)[r0 + tid];
     sbias[tid] = b;
   }
   G16Acc<NP, CFG> acc;
-  g16_tile<NP, CFG, false, false>(acc, p.w, p.x, r0, c0, 0, p.Dp, lds);
-  const float ix = NP == 2 ? 1.f / p.scale[0] : 1.f, iw = NP == 2 ? 1.f / p.scale[1] : 1.f;       // powers of two: exact
+  float* z = nullptr;                                     // (waves of no row have nothing to keep)
+  if (p.z && c0 + g16_c<CFG>(wc, 0, 0) < n)
+    z = p.z + (((int64_t)tr * p.tiles_c + tc) * (g16_nt(CFG) / 64) + wid) * (C::RB * C::CB * 1024) + lane * 4;
+  if (GRAD && p.z) {
 #pragma unroll
-  for (int i = 0; i < C::RB; ++i)
-#pragma unroll
-    for (int eb = 0; eb < 4; ++eb) {
-      const float4 b = *reinterpret_cast<const float4*>(sbias + g16_r<CFG>(wr, i, eb * 4, lane));
-      const float bb[4] = {b.x, b.y, b.z, b.w};
+    for (int i = 0; i < C::RB; ++i)
 #pragma unroll
       for (int j = 0; j < C::CB; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][eb * 4 + e] = (NP == 2 ? acc[i][j][eb * 4 + e] * ix * iw : acc[i][j][eb * 4 + e]) + bb[e];
-    }
-  const int nv = p.V - r0;                                      // rows of this tile inside the vocabulary
-  int yl[C::CB];                                                    // the target's row in this tile, or none
+        for (int eb = 0; eb < 4; ++eb) {
+          const float4 v = z ? *reinterpret_cast<const float4*>(z + ((i * C::CB + j) * 4 + eb) * 256) : make_float4(0.f, 0.f, 0.f, 0.f);
+          acc[i][j][eb * 4] = v.x; acc[i][j][eb * 4 + 1] = v.y; acc[i][j][eb * 4 + 2] = v.z; acc[i][j][eb * 4 + 3] = v.w;
+        }
+    __syncthreads();
+  } else {
+    g16_tile<NP, CFG, false, false>(acc, p.w, p.x, r0, c0, 0, p.Dp, lds);
+  }
+  if (!GRAD && z) {
+#pragma unroll
+    for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+      for (int j = 0; j < C::CB; ++j)
+#pragma unroll
+        for (int eb = 0; eb < 4; ++eb)
+          *reinterpret_cast<float4*>(z + ((i * C::CB + j) * 4 + eb) * 256) =
+              make_float4(acc[i][j][eb * 4], acc[i][j][eb * 4 + 1], acc[i][j][eb * 4 + 2], acc[i][j][eb * 4 + 3]);
+  }
+  // What few tiles need (a bias, rows past the vocabulary, a target) is passed over as a whole where it is not there: the epilogue of
+  // 256 x 256 logits takes a wave's instructions as long as three k-steps.
+  if constexpr (NP == 2) {
+    const float ix = 1.f / p.scale[0], iw = 1.f / p.scale[1];       // powers of two: exact
+#pragma unroll
+    for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+      for (int j = 0; j < C::CB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i][j][e] * ix * iw;
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+      for (int eb = 0; eb < 4; ++eb) {
+        const float4 b = *reinterpret_cast<const float4*>(sbias + g16_r<CFG>(wr, i, eb * 4, lane));
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < C::CB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][eb * 4 + e] += bb[e];
+      }
+  }
+  const int nv = p.V - r0;                                          // rows of this tile inside the vocabulary
+  int yl[C::CB];                                                    // the target's row in this tile where this lane holds it, or -1
 #pragma unroll
   for (int j = 0; j < C::CB; ++j) {
     const int c = c0 + g16_c<CFG>(wc, j, lane);
-    const int64_t y = c < p.T ? p.y[c] : -1;
-    yl[j] = y >= r0 && y < r0 + TL && y < p.V ? (int)(y - r0) : -1;
+    const int y = (c < n ? p.rows.y[c] : -1) - r0;
+    yl[j] = y >= 0 && y < TL && y / (C::RB * 32) == wr && (y >> 2 & 1) == lh && y < nv ? y : -1;
   }
   if constexpr (!GRAD) {
+    if (nv < TL) {
+#pragma unroll
+      for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+        for (int j = 0; j < C::CB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = g16_r<CFG>(wr, i, e, lane) < nv ? acc[i][j][e] : -INFINITY;
+    }
 #pragma unroll
     for (int j = 0; j < C::CB; ++j) {
-      float m = -INFINITY, z = 0.f;
+      float m = -INFINITY, s = 0.f, t = 0.f;
+      // the largest that is no NaN; a NaN gets into the sum of exponentials by itself
 #pragma unroll
       for (int i = 0; i < C::RB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = g16_r<CFG>(wr, i, e, lane);
-          const float v = acc[i][j][e];
-          if (r < nv) { m = v > m || v != v ? v : m; z += v; }
-          if (r == yl[j]) p.zy[c0 + g16_c<CFG>(wc, j, lane)] = v;
-        }
-      const float om = __shfl_xor(m, 32, 64);
-      m = om > m || om != om ? om : m;
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float safe = m == -INFINITY ? 0.f : m;
-      float s = 0.f;
 #pragma unroll
       for (int i = 0; i < C::RB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += g16_r<CFG>(wr, i, e, lane) < nv ? __expf(acc[i][j][e] - safe) : 0.f;
+        for (int e = 0; e < 16; ++e) s += __expf(acc[i][j][e] - safe);
       s += __shfl_xor(s, 32, 64);
-      z += __shfl_xor(z, 32, 64);
+      if (p.zsum) {
+#pragma unroll
+        for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) t += g16_r<CFG>(wr, i, e, lane) < nv ? acc[i][j][e] : 0.f;
+        t += __shfl_xor(t, 32, 64);
+      }
+      if (__any(yl[j] >= 0)) {
+        float zy = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zy = g16_r<CFG>(wr, i, e, lane) == yl[j] ? acc[i][j][e] : zy;
+        if (yl[j] >= 0) p.zy[c0 + g16_c<CFG>(wc, j, lane)] = zy;
+      }
       if (lh == 0) {
         const int c = g16_c<CFG>(wc, j, lane);
-        stat[0][wr][c] = m; stat[1][wr][c] = s; stat[2][wr][c] = z;
+        stat[0][wr][c] = m; stat[1][wr][c] = s; stat[2][wr][c] = t;
       }
     }
     __syncthreads();
-    if (tid < TL && c0 + tid < p.T) {
+    if (tid < TL && c0 + tid < n) {
       const float m0 = stat[0][0][tid], m1 = stat[0][1][tid];
-      const float m = m1 > m0 || m1 != m1 ? m1 : m0;
+      const float m = fmaxf(m0, m1);
       const float safe = m == -INFINITY ? 0.f : m;
       const float s = stat[1][0][tid] * __expf(m0 - safe) + stat[1][1][tid] * __expf(m1 - safe);
       const int64_t at = (int64_t)tr * p.Tp + c0 + tid;
@@ -253,23 +406,34 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
       if (p.zsum) p.zsum[at] = stat[2][0][tid] + stat[2][1][tid];
     }
   } else {
-    float w[C::CB], lse[C::CB];
-    const float uni = p.g.reduction ? ce_uniform(p.g) : 0.f, gs = ce_gscale<NP>(p.g);
+    const float unit = 1.f / ce_unit(p.eps), gs = p.g.reduction ? ce_gscale<NP>() : ce_gscale<NP>() / p.g.shared[0];
+    const float ev = p.eps / (float)p.V * unit, on = (1.f - p.eps) * unit;
 #pragma unroll
     for (int j = 0; j < C::CB; ++j) {
       const int c = c0 + g16_c<CFG>(wc, j, lane);
-      const int64_t y = c < p.T ? p.y[c] : p.ignore;
-      w[j] = y == p.ignore || y < 0 || y >= p.V ? 0.f : (p.g.reduction ? uni : p.g.grad[c]) * gs;
-      lse[j] = c < p.T ? p.lse[c] : 0.f;
+      const bool live = c < n && p.rows.y[c] >= 0;
+      const float w = !live ? 0.f : p.g.reduction ? gs : p.g.grad[p.rows.idx[c]] * gs, lse = live ? p.rows.lse[c] : 0.f;
+      const float wu = w * unit, we = -ev * w, wy = -on * w;
+#pragma unroll
+      for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(__expf(acc[i][j][e] - lse), wu, we);
+      if (__any(yl[j] >= 0)) {
+#pragma unroll
+        for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] += g16_r<CFG>(wr, i, e, lane) == yl[j] ? wy : 0.f;
+      }
+      if (nv < TL || __any(w == 0.f)) {
+#pragma unroll
+        for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = g16_r<CFG>(wr, i, e, lane) < nv && w != 0.f ? acc[i][j][e] : 0.f;
+      }
     }
     float colsum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float ev = p.eps / (float)p.V, on = 1.f - p.eps;
     g16_store_tile<NP, CFG, false>(
-        [&](int i, int j, int e) {
-          const int r = g16_r<CFG>(wr, i, e, lane);
-          const float g = (__expf(acc[i][j][e] - lse[j]) - (r == yl[j] ? on : 0.f) - ev) * w[j];
-          return r < nv && w[j] != 0.f ? g : 0.f;
-        },
+        [&](int i, int j, int e) { return acc[i][j][e]; },
         [&](int c, int r, const float (&v)[8]) {
           const int64_t row = c0 + c, col = tr * TL + r;
           if constexpr (DB) {
@@ -309,36 +473,28 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
 // Joins the tiles' statistics, TOK tokens to a workgroup a time and NT / TOK threads to a token; ONE: one workgroup for all of it, and with
 // it the reduction.
 struct CeJoin {
-  const float2* part; const float* zsum; const float* zy; const int64_t* y;
-  int64_t ignore, Tp;
-  int T, V, tiles, reduction;
+  const float2* part; const float* zsum; const float* zy;
+  CeRows k;
+  int64_t Tp;
+  int V, tiles, reduction;
   float eps;
-  float* lse; float* rows; float* loss; float* scale;
+  float* rows; float* loss;                          // rows: losses of the packed rows; reduction none: loss, of all rows
 };
 
-// number of live rows and, for mean / sum, the loss: one workgroup, a fixed order
+// the loss of mean / sum: one workgroup, a fixed order
 template <int NT>
 __device__ __forceinline__ void ce_reduce(const CeJoin& p) {
   __shared__ double rs[NT / 64];
-  __shared__ int rn[NT / 64];
+  const int n = *p.k.n;
   double s = 0.0;
-  int n = 0;
-  for (int t = threadIdx.x; t < p.T; t += NT) {
-    s += p.rows[t];
-    n += p.y[t] != p.ignore;
-  }
+  for (int t = threadIdx.x; t < n; t += NT) s += p.rows[t];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    s += __shfl_xor(s, o, 64);
-    n += __shfl_xor(n, o, 64);
-  }
-  if ((threadIdx.x & 63) == 0) { rs[threadIdx.x >> 6] = s; rn[threadIdx.x >> 6] = n; }
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) rs[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < NT / 64; ++i) { s += rs[i]; n += rn[i]; }
-    p.scale[2] = (float)n;
-    if (p.reduction == 1) *p.loss = (float)(s / (double)n);      // no live row: 0 / 0, a NaN, as a mean over nothing is
-    else if (p.reduction == 2) *p.loss = (float)s;
+    for (int i = 1; i < NT / 64; ++i) s += rs[i];
+    *p.loss = (float)(p.reduction == 1 ? s / (double)n : s);        // no row: 0 / 0, a NaN, as a mean over nothing is
   }
 }
 
@@ -347,13 +503,14 @@ __global__ __launch_bounds__(NT) void ce_join_kernel(CeJoin p) {
   constexpr int PER = NT / TOK;
   __shared__ float sm[3][PER][TOK];
   const int l = threadIdx.x % TOK, q = threadIdx.x / TOK;
-  for (int t0 = blockIdx.x * TOK; t0 < p.T; t0 += gridDim.x * TOK) {
+  const int n = *p.k.n;
+  for (int t0 = blockIdx.x * TOK; t0 < n; t0 += gridDim.x * TOK) {
     const int t = t0 + l;
     float m = -INFINITY, s = 0.f, z = 0.f;
-    if (t < p.T)
+    if (t < n)
       for (int k = q; k < p.tiles; k += PER) {
         const float2 v = p.part[(int64_t)k * p.Tp + t];
-        const float nm = v.x > m || v.x != v.x ? v.x : m;
+        const float nm = fmaxf(m, v.x);
         const float safe = nm == -INFINITY ? 0.f : nm;
         s = s * __expf(m - safe) + v.y * __expf(v.x - safe);
         m = nm;
@@ -365,7 +522,7 @@ __global__ __launch_bounds__(NT) void ce_join_kernel(CeJoin p) {
       __syncthreads();
       if (q < half) {
         const float om = sm[0][q + half][l];
-        const float nm = om > m || om != om ? om : m;
+        const float nm = fmaxf(m, om);
         const float safe = nm == -INFINITY ? 0.f : nm;
         s = s * __expf(m - safe) + sm[1][q + half][l] * __expf(om - safe);
         m = nm;
@@ -373,47 +530,43 @@ __global__ __launch_bounds__(NT) void ce_join_kernel(CeJoin p) {
         sm[0][q][l] = m; sm[1][q][l] = s; sm[2][q][l] = z;
       }
     }
-    if (q == 0 && t < p.T) {
+    if (q == 0 && t < n) {
       const float L = m + logf(s);
-      const int64_t yt = p.y[t];
-      float loss;
-      if (yt == p.ignore) loss = 0.f;
-      else if (yt < 0 || yt >= p.V) loss = NAN;               // a target outside the vocabulary: loud, but no read out of range
-      else {
+      float loss = NAN;                              // a target outside the vocabulary: loud, but no read out of range
+      if (p.k.y[t] >= 0) {
         loss = L - (1.f - p.eps) * p.zy[t];
         if (p.eps != 0.f) loss -= p.eps * (z / (float)p.V);
       }
-      p.lse[t] = L;
-      p.rows[t] = loss;
+      p.k.lse[t] = L;
+      if (p.reduction) p.rows[t] = loss;
+      else p.loss[p.k.idx[t]] = loss;
     }
   }
   if constexpr (ONE) {
     __syncthreads();
-    ce_reduce<NT>(p);
+    if (p.reduction) ce_reduce<NT>(p);
   }
 }
 __global__ __launch_bounds__(1024) void ce_reduce_kernel(CeJoin p) { ce_reduce<1024>(p); }
 
-// The power of two for rows with gradients of their own, two planes: one workgroup
-__global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict__ grad, const int64_t* __restrict__ y, int64_t ignore, int T,
-                                                         int V, float* __restrict__ shared) {
+// The largest of rows' own gradients (1 where that is 0, Inf, NaN or has no reciprocal): one workgroup
+__global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict__ grad, CeRows k, float* __restrict__ shared) {
   __shared__ float red[16];
   float m = 0.f;
-  for (int64_t t = threadIdx.x; t < T; t += 1024) {
-    const int64_t yt = y[t];
-    if (yt != ignore && yt >= 0 && yt < V) m = fmaxf(m, fabsf(grad[t]));
-  }
+  for (int t = threadIdx.x; t < *k.n; t += 1024)
+    if (k.y[t] >= 0) m = fmaxf(m, fabsf(grad[k.idx[t]]));
   m = ofq_wave_max(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-    shared[0] = ce_scale(m);
+    shared[0] = m >= 1e-37f && m <= 1e37f ? m : 1.f;
   }
 }
 
 struct CeOut {
   G16Op P, Q;
+  CeRows rows;
   const unsigned short* tail;              // dx: P's last G16_PAD rows of k where K ends in front of them, or NULL
   int R, C, K, tiles_r, tiles_c, split;
   float* part; int64_t slot;               // fp32 [split][C][R], accumulated into where acc is set
@@ -441,33 +594,36 @@ __device__ __forceinline__ void ce_put(void* out, int out16, int64_t at, int n, 
   }
 }
 
-// dx (QCOL false: P = W [k = v][r = d], Q = G [c = t][k = v]) and dW (QCOL true: P = x [k = t][r = d], Q = G [k = t][c = v])
+// dx (QCOL false: P = W [k = v][r = d], Q = G [c = t][k = v]) and dW (QCOL true: P = x [k = t][r = d], Q = G [k = t][c = v]); t: packed rows.
+// A part of a split k has consecutive workgroups of one XCD, so that they take whole rows of W.
 template <int NP, int CFG, bool QCOL>
 __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
   using C = G16<NP, CFG>;
   G16_SHARED(NP, CFG)
+  const int id = g16_xcd(blockIdx.x, gridDim.x, gridDim.x), tiles = p.tiles_r * p.tiles_c, sp = id / tiles, n = *p.rows.n;
   int tr, tc;
-  g16_group(g16_xcd(blockIdx.x, gridDim.x, gridDim.x), p.tiles_r, p.tiles_c, tr, tc);
+  g16_group(id - sp * tiles, p.tiles_r, p.tiles_c, tr, tc);
+  if (!QCOL && tc * C::T >= n) return;
   constexpr int BK = C::BK;
-  const int nk = p.K / BK, per = (nk + p.split - 1) / p.split;
-  const int kb = min((int)blockIdx.y * per, nk), ke = min(kb + per, nk);
+  const int nk = (QCOL ? ce_padded(n) : p.K) / BK, per = (nk + p.split - 1) / p.split;
+  const int kb = min(sp * per, nk), ke = min(kb + per, nk);
   G16Acc<NP, CFG> acc;
   g16_tile<NP, CFG, true, QCOL>(acc, p.P, p.Q, tr * C::T, tc * C::T, kb * BK, ke * BK, lds);
   if constexpr (!QCOL) {
-    if (p.tail && blockIdx.y + 1 == p.split) {
+    if (p.tail && sp + 1 == p.split) {
       const G16Op tp = {p.tail, p.P.ld, 0, G16_PAD, p.P.cols}, tq = {p.Q.p + p.K, p.Q.ld, p.Q.plane, p.Q.rows, p.Q.cols};
       g16_tile<NP, CFG, true, false, true>(acc, tp, tq, tr * C::T, tc * C::T, 0, G16_PAD, lds);
     }
   }
-  const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = NP == 2 ? 1.f / ce_gscale<NP>(p.g) : 1.f;
+  const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = ce_factor<NP>(p.g);
   g16_store_tile<NP, CFG, false>([&](int i, int j, int e) { return acc[i][j][e]; },
                  [&](int c, int r, const float (&v0)[8]) {
                    const int64_t row = tc * C::T + c;
                    const int col = tr * C::T + r;
-                   if (row >= p.C || col >= p.R) return;
+                   if (row >= (QCOL ? p.C : n) || col >= p.R) return;
                    float v[8];
                    if (p.part) {
-                     float* o = p.part + blockIdx.y * p.slot + row * p.R + col;       // R and slot are multiples of 64
+                     float* o = p.part + sp * p.slot + row * p.R + col;       // R and slot are multiples of 64
 #pragma unroll
                      for (int e = 0; e < 8; ++e) v[e] = v0[e];
                      if (p.acc) {
@@ -477,55 +633,59 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
                      ce_put(o, 0, 0, 8, v);
                    } else {
 #pragma unroll
-                     for (int e = 0; e < 8; ++e) v[e] = v0[e] * a * b;
-                     ce_put(p.out, p.out16, row * p.ldo + col, p.R - col, v);
+                     for (int e = 0; e < 8; ++e) v[e] = ce_times(v0[e] * a, b);
+                     ce_put(p.out, p.out16, (QCOL ? row : (int64_t)p.rows.idx[row]) * p.ldo + col, p.R - col, v);
                    }
                  },
                  [](int, int, const float (&)[8]) {}, lds);
 }
 
-// dx = sum of the split's partials, in order, scaled and typed
+// dx = sum of the split's partials, in order, scaled and typed, and zeros in the rows that do not count; part NULL: those alone
 template <int NP>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, const float* __restrict__ scale,
-                                                    CeGrad g, void* __restrict__ dx, int out16) {
+                                                    CeRows k, CeGrad g, void* __restrict__ dx, int out16) {
   const int64_t per = d.Dp / 8, n = d.T * per;
-  const float a = NP == 2 ? 1.f / scale[0] : 1.f, b = NP == 2 ? 1.f / ce_gscale<NP>(g) : 1.f;
+  const float a = NP == 2 ? 1.f / scale[0] : 1.f, b = ce_factor<NP>(g);
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t t = i / per, c = (i - t * per) * 8;
     if (c >= d.D) continue;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float* p = part + t * d.Dp + c;
+    const int at = k.pos[t];
+    if (at >= 0 && !part) continue;
+    const float* p = part + at * d.Dp + c;
+    const int ns = at < 0 ? 0 : split;
 #pragma unroll 8
-    for (int s = 0; s < split; ++s) {
+    for (int s = 0; s < ns; ++s) {
       const float4 x = *reinterpret_cast<const float4*>(p + s * slot), y = *reinterpret_cast<const float4*>(p + s * slot + 4);
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * a * b;
+    for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e] * a, b);
     ce_put(dx, out16, t * d.D + c, (int)min((int64_t)8, d.D - c), v);
   }
 }
 
-// the bias gradient from the tiles' column sums, in order
+// the bias gradient from the sums of columns of ce_padded(n) / TL tiles, in order
 template <int NP>
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int64_t ldg, int ny, int n, CeGrad g, void* __restrict__ db,
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int64_t ldg, int TL, int n, CeGrad g, void* __restrict__ db,
                                                     int out16, int64_t at) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= n) return;
   float s = 0.f;
+  const int ny = (ce_padded(*g.n) + TL - 1) / TL;
 #pragma unroll 8
   for (int k = 0; k < ny; ++k) s += part[k * ldg + c];
-  s *= NP == 2 ? 1.f / ce_gscale<NP>(g) : 1.f;
+  s = ce_times(s, ce_factor<NP>(g));
   if (out16) reinterpret_cast<unsigned short*>(db)[at + c] = g16_bf16(s);
   else reinterpret_cast<float*>(db)[at + c] = s;
 }
 
 static int ce_w_aligned(const void* w) { return ((uintptr_t)w & 15) == 0; }
 
-extern "C" size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned) {
+extern "C" size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, int backward) {
   CeDims d;
   if (!ce_dims(T, D, V, bf16, w_aligned, &d)) return 0;
-  return ce_kept(nullptr, d).bytes;
+  return ce_kept(nullptr, d, backward != 0).bytes;
 }
 
 struct CeFwdWs { float* amax; float2* part; float* zsum; float* zy; float* rows; size_t bytes; };
@@ -556,8 +716,7 @@ static G16Op ce_w_op(const CeDims& d, const CeKept& k, const void* w, int64_t v0
 // launches with the tile form of their grid: logits of V' columns (tv: tiles along them), gradient products
 template <bool GRAD>
 static int ce_logits(CeLogits& a, int64_t V, int64_t T, int bf16, int* tv, hipStream_t st) {
-  auto tiles = [&](int t) { return ceil_div(V, t) * ceil_div(T, t); };
-  const int form = g16_form(tiles(64), tiles(128), tiles(256)), t = g16_t(form);
+  const int form = ce_form(V, T, 1), t = g16_t(form);
   a.tiles_r = (int)ceil_div(V, t); a.tiles_c = (int)ceil_div(T, t);
   if (tv) *tv = a.tiles_r;
   const dim3 g((unsigned)(a.tiles_r * a.tiles_c));
@@ -574,10 +733,9 @@ static int ce_logits(CeLogits& a, int64_t V, int64_t T, int bf16, int* tv, hipSt
 }
 template <bool QCOL>
 static int ce_grad(CeOut& o, int bf16, hipStream_t st) {
-  auto tiles = [&](int t) { return ceil_div(o.R, t) * ceil_div(o.C, t) * o.split; };
-  const int form = g16_form(tiles(64), tiles(128), tiles(256)), t = g16_t(form);
+  const int form = ce_form(o.R, o.C, o.split), t = g16_t(form);
   o.tiles_r = (int)ceil_div(o.R, t); o.tiles_c = (int)ceil_div(o.C, t);
-  const dim3 g((unsigned)(o.tiles_r * o.tiles_c), (unsigned)o.split);
+  const dim3 g((unsigned)(o.tiles_r * o.tiles_c * o.split));
 #define CE_GRAD(NP, CFG) hipLaunchKernelGGL((ce_grad_kernel<NP, CFG, QCOL>), g, dim3(g16_nt(CFG)), 0, st, o)
   if (bf16) { if (form == G16_BIG) CE_GRAD(1, G16_BIG); else if (form == G16_MID) CE_GRAD(1, G16_MID); else if (form == G16_DEEP) CE_GRAD(1, G16_DEEP); else CE_GRAD(1, G16_TINY); }
   else { if (form == G16_BIG) CE_GRAD(2, G16_BIG); else if (form == G16_MID) CE_GRAD(2, G16_MID); else if (form == G16_DEEP) CE_GRAD(2, G16_DEEP); else CE_GRAD(2, G16_TINY); }
@@ -588,38 +746,37 @@ static int ce_grad(CeOut& o, int bf16, hipStream_t st) {
 
 // reduction: 0 none (loss [T]), 1 mean, 2 sum (loss: one float)
 extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
-                                 int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, float* loss, float* lse,
+                                 int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, int backward, float* loss,
                                  void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, ofq_stream_t stream) {
   CeDims d;
-  if (!x || !w || !target || !loss || !lse || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
+  if (!x || !w || !target || !loss || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
       !ce_dims(T, D, V, bf16, ce_w_aligned(w), &d) || ((uintptr_t)kept & 255) || ((uintptr_t)ws & 255))
     return OFQ_EINVAL;
-  const CeKept k = ce_kept(kept, d);
+  const CeKept k = ce_kept(kept, d, backward != 0);
   const CeFwdWs f = ce_fwd_ws(ws, d);
   if (kept_bytes < k.bytes || ws_bytes < f.bytes) return OFQ_ENOWS;
   const int64_t tiles = d.tiles_v * d.tiles_t;
   if (tiles >= (1ll << 31)) return OFQ_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  if (!bf16) {
-    hipLaunchKernelGGL(ce_amax_kernel, dim3(CE_AMAX_X + CE_AMAX_W), dim3(256), 0, st, (const float*)x, target, ignore_index, T, D,
-                       (const float*)w, V * D, f.amax);
-    OFQ_LAUNCH_CHECK();
-  }
+  float* rows_out = reduction == 0 ? loss : nullptr;
+  if (bf16) hipLaunchKernelGGL(ce_number_kernel, dim3(1), dim3(1024), 0, st, target, ignore_index, T, (int)V, k.rows, rows_out);
+  else hipLaunchKernelGGL(ce_amax_kernel, dim3(CE_AMAX_X + CE_AMAX_W + 1), dim3(256), 0, st, (const float*)x, target, ignore_index, T, D,
+                          (int)V, (const float*)w, V * D, f.amax, k.rows, rows_out);
+  OFQ_LAUNCH_CHECK();
   const int64_t chunks = (d.Tp + ce_w_rows(d)) * (d.Dp / 8);
   const dim3 pg((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 4096));
-  if (bf16) hipLaunchKernelGGL(ce_pack_kernel<1>, pg, dim3(256), 0, st, x, target, ignore_index, w, d, f.amax, k);
-  else hipLaunchKernelGGL(ce_pack_kernel<2>, pg, dim3(256), 0, st, x, target, ignore_index, w, d, f.amax, k);
+  if (bf16) hipLaunchKernelGGL(ce_pack_kernel<1>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
+  else hipLaunchKernelGGL(ce_pack_kernel<2>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
   OFQ_LAUNCH_CHECK();
   CeLogits a = {};
   a.w = ce_w_op(d, k, w, 0);
   a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
-  a.bias = bias; a.bias16 = bias16; a.y = target; a.ignore = ignore_index; a.scale = k.scale;
-  a.T = (int)T; a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing;
+  a.rows = k.rows; a.bias = bias; a.bias16 = bias16; a.scale = k.scale; a.z = k.z;
+  a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing;
   a.part = f.part; a.zsum = smoothing != 0.f ? f.zsum : nullptr; a.zy = f.zy;
   int tv;
   if (int rc = ce_logits<false>(a, V, T, bf16, &tv, st)) return rc;
-  const CeJoin j = {f.part, a.zsum, f.zy, target, ignore_index, d.Tp, (int)T, (int)V, tv, reduction, smoothing, lse,
-                    reduction == 0 ? loss : f.rows, loss, k.scale};
+  const CeJoin j = {f.part, a.zsum, f.zy, k.rows, d.Tp, (int)V, tv, reduction, smoothing, f.rows, loss};
   // little to join: one workgroup does that and the sum, one launch less
   if (T * tv <= 8192) {
     if (tv <= 64) hipLaunchKernelGGL((ce_join_kernel<1024, 128, true>), dim3(1), dim3(1024), 0, st, j);
@@ -627,7 +784,7 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   } else {
     hipLaunchKernelGGL((ce_join_kernel<256, 8, false>), dim3((unsigned)std::min<int64_t>(ceil_div(T, 8), 65536)), dim3(256), 0, st, j);
     OFQ_LAUNCH_CHECK();
-    hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, j);
+    if (reduction) hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, j);
   }
   OFQ_LAUNCH_CHECK();
   return 0;
@@ -636,11 +793,7 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
 struct CeBwd { int64_t piece, pieces; int split; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
 static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) {
   CeBwd b;
-  const int64_t vp = ceil_div(d.V, 128) * 128;
-  b.piece = std::min(vp, std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.np) / 128 * 128, 128));
-  b.pieces = ceil_div(vp, b.piece);
-  b.piece = ceil_div(ceil_div(vp, b.pieces), 128) * 128;             // pieces of one size
-  b.pieces = ceil_div(vp, b.piece);
+  b.pieces = ce_pieces(d, &b.piece);
   // dx has few tiles and a long k: split it until two workgroups to a CU have work, at no less than eight k-steps each
   const int64_t tiles = ceil_div(d.T, 128) * ceil_div(d.D, 128), steps = b.piece / (d.np == 1 ? 64 : 32);
   b.split = tiles >= 384 ? 1 : (int)std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 8));
@@ -662,23 +815,22 @@ extern "C" size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, in
   return ce_bwd_ws(nullptr, d, want_dx != 0, want_db != 0).bytes;
 }
 
-// grad: the incoming gradient, one float or (reduction 0) [T]; lse and kept as the forward pass left them; dx / dw / db: any may be NULL
-extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const int64_t* target, const float* lse, const void* kept,
-                                 int64_t T, int64_t D, int64_t V, int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction,
-                                 void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream) {
+// grad: the incoming gradient, one float or (reduction 0) [T]; kept as a forward pass with backward != 0 left it; dx / dw / db: any may be NULL
+extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, int64_t T, int64_t D, int64_t V,
+                                 int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream) {
   CeDims d;
-  if (!grad || !w || !target || !lse || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
+  if (!grad || !w || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
       !ce_dims(T, D, V, bf16, ce_w_aligned(w), &d) || ((uintptr_t)kept & 255) || ((uintptr_t)ws & 255))
     return OFQ_EINVAL;
-  const CeKept k = ce_kept((void*)kept, d);
+  const CeKept k = ce_kept((void*)kept, d, true);
   const CeBwd b = ce_bwd_ws(ws, d, dx != nullptr, db != nullptr);
   if (ws_bytes < b.bytes) return OFQ_ENOWS;
   hipStream_t st = (hipStream_t)stream;
-  if (reduction == 0 && d.np == 2) {
-    hipLaunchKernelGGL(ce_weight_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore_index, (int)T, (int)V, b.shared);
+  if (reduction == 0) {
+    hipLaunchKernelGGL(ce_weight_kernel, dim3(1), dim3(1024), 0, st, grad, k.rows, b.shared);
     OFQ_LAUNCH_CHECK();
   }
-  const CeGrad cg = {grad, k.scale, b.shared, reduction};
+  const CeGrad cg = {grad, k.rows.n, b.shared, reduction, smoothing};
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, V - v0);
     const bool tail = !d.pack_w && nv % G16_PAD;                          // (of the last piece: the others are whole tiles)
@@ -686,13 +838,14 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     CeLogits a = {};
     a.w = ce_w_op(d, k, w, 0);
     a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
-    a.bias = bias; a.bias16 = bias16; a.y = target; a.ignore = ignore_index; a.scale = k.scale;
-    a.T = (int)T; a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing; a.v0 = (int)v0;
-    a.lse = lse; a.g = cg; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
+    a.rows = k.rows; a.bias = bias; a.bias16 = bias16; a.scale = k.scale; a.z = k.z;
+    a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing; a.v0 = (int)v0;
+    a.g = cg; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
     if (int rc = ce_logits<true>(a, nv, T, bf16, nullptr, st)) return rc;
     const int64_t gpl = d.Tp * b.piece;
     if (dw) {
       CeOut o = {};
+      o.rows = k.rows;
       o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.R = (int)D; o.C = (int)nv; o.K = (int)d.Tp; o.split = 1;
@@ -701,6 +854,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     }
     if (dx) {
       CeOut o = {};
+      o.rows = k.rows;
       o.P = ce_w_op(d, k, w, v0);
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.C = (int)T; o.K = (int)kdx; o.split = b.split; o.tail = tail ? k.w : nullptr; o.scale = k.scale + 1; o.g = cg;
@@ -710,15 +864,16 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     }
     if (db) {
       const dim3 g((unsigned)ceil_div(nv, 256));
-      if (bf16) hipLaunchKernelGGL(ce_db_kernel<1>, g, dim3(256), 0, st, b.db, b.piece, a.tiles_c, (int)nv, cg, db, bias16, v0);
-      else hipLaunchKernelGGL(ce_db_kernel<2>, g, dim3(256), 0, st, b.db, b.piece, a.tiles_c, (int)nv, cg, db, bias16, v0);
+      const int tl = g16_t(ce_form(nv, T, 1));
+      if (bf16) hipLaunchKernelGGL(ce_db_kernel<1>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, db, bias16, v0);
+      else hipLaunchKernelGGL(ce_db_kernel<2>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, db, bias16, v0);
       OFQ_LAUNCH_CHECK();
     }
   }
-  if (dx && b.part) {
+  if (dx) {
     const dim3 g((unsigned)std::min<int64_t>(ceil_div(T * (d.Dp / 8), 256), 8192));
-    if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, cg, dx, bf16);
-    else hipLaunchKernelGGL(ce_dx_kernel<2>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, cg, dx, bf16);
+    if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
+    else hipLaunchKernelGGL(ce_dx_kernel<2>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
     OFQ_LAUNCH_CHECK();
   }
   return 0;

@@ -1308,8 +1308,9 @@ class AssembleTokensFn(torch.autograd.Function):
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
-    """Cross entropy of x @ weight^T + bias against integer targets, logits never kept (csrc/linear_ce.hip).  The forward leaves the
-    log-sum-exp of every row and the operands' 16-bit planes; the backward recomputes the logits a piece of the vocabulary at a time."""
+    """Cross entropy of x @ weight^T + bias against integer targets (csrc/linear_ce.hip).  The forward leaves the log-sum-exp of every
+    row that counts, the operands' 16-bit planes and up to 128 MB of logits; where they are more, the backward recomputes them, a
+    piece of the vocabulary at a time."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, smoothing, reduction):
@@ -1319,20 +1320,20 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
         with ops.on_device(x.device):
-            loss, lse, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red)
-        ctx.save_for_backward(w, b, y, lse, kept)
-        ctx.args = (x.shape, D, ignore_index, smoothing, red, int(x.dtype == torch.bfloat16))
+            loss, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(w, b, kept)
+        ctx.args = (x.shape, y.numel(), smoothing, red)
         return loss.view(target.shape) if red == 0 else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        w, b, y, lse, kept = ctx.saved_tensors
-        shape, D, ignore_index, smoothing, red, b16 = ctx.args
+        w, b, kept = ctx.saved_tensors
+        shape, T, smoothing, red = ctx.args
         need = ctx.needs_input_grad
         with ops.on_device(w.device):
-            dx, dw, db = ops.linear_ce_bwd(g.reshape(-1).contiguous(), w, b, y, lse, kept, D, ignore_index, smoothing, red, b16,
-                                           want_dx=need[0], want_dw=need[1], want_db=need[2])
+            dx, dw, db = ops.linear_ce_bwd(g.reshape(-1).contiguous(), w, b, kept, T, smoothing, red, want_dx=need[0], want_dw=need[1],
+                                           want_db=need[2])
         return dx.view(shape) if dx is not None else None, dw, db, None, None, None, None
 
 

@@ -1443,36 +1443,35 @@ def _scratch(nbytes, device):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
 
 
-def linear_ce_fwd(x2d, weight, bias, target, ignore_index, smoothing, reduction):
-    """(loss, lse, kept): loss [T] or a scalar, lse [T], both fp32; kept: the operands' planes, for linear_ce_bwd."""
+def linear_ce_fwd(x2d, weight, bias, target, ignore_index, smoothing, reduction, backward=True):
+    """(loss, kept): loss [T] or a scalar, fp32; kept: what linear_ce_bwd needs beside its arguments (where one is to come)."""
     T, D = x2d.shape
     V = weight.shape[0]
     dev, b16 = x2d.device, int(x2d.dtype == torch.bfloat16)
     L = lib()
-    kept = _scratch(L.ofq_linear_ce_kept_bytes(T, D, V, b16, int(weight.data_ptr() % 16 == 0)), dev)
+    kept = _scratch(L.ofq_linear_ce_kept_bytes(T, D, V, b16, int(weight.data_ptr() % 16 == 0), int(backward)), dev)
     ws = _scratch(L.ofq_linear_ce_fwd_ws_bytes(T, D, V, b16), dev)
     loss = torch.empty((T,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-    lse = torch.empty(T, dtype=torch.float32, device=dev)
     with _Timed("linear cross entropy, forward", 2.0 * T * D * V):
         _chk(L.ofq_linear_ce_fwd(x2d.data_ptr(), weight.data_ptr(), _p(bias), target.data_ptr(), T, D, V, b16,
                                  int(bias is not None and bias.dtype == torch.bfloat16), ignore_index, smoothing, reduction,
-                                 loss.data_ptr(), lse.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(), ws.numel(), _stream()),
+                                 int(backward), loss.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(), ws.numel(), _stream()),
              "ofq_linear_ce_fwd")
-    return loss, lse, kept
+    return loss, kept
 
 
-def linear_ce_bwd(grad, weight, bias, target, lse, kept, D, ignore_index, smoothing, reduction, b16, want_dx=True, want_dw=True,
-                  want_db=True):
-    T, V, dev = target.numel(), weight.shape[0], weight.device
+def linear_ce_bwd(grad, weight, bias, kept, T, smoothing, reduction, want_dx=True, want_dw=True, want_db=True):
+    V, D = weight.shape
+    dev, b16 = weight.device, int(weight.dtype == torch.bfloat16)
     L = lib()
     dx = torch.empty((T, D), dtype=weight.dtype, device=dev) if want_dx else None
     dw = torch.empty_like(weight) if want_dw else None
     db = torch.empty_like(bias) if want_db and bias is not None else None
     ws = _scratch(L.ofq_linear_ce_bwd_ws_bytes(T, D, V, b16, int(dx is not None), int(db is not None)), dev)
     with _Timed("linear cross entropy, backward", 6.0 * T * D * V):
-        _chk(L.ofq_linear_ce_bwd(grad.data_ptr(), weight.data_ptr(), _p(bias), target.data_ptr(), lse.data_ptr(), kept.data_ptr(),
-                                 T, D, V, b16, int(bias is not None and bias.dtype == torch.bfloat16), ignore_index, smoothing,
-                                 reduction, _p(dx), _p(dw), _p(db), ws.data_ptr(), ws.numel(), _stream()),
+        _chk(L.ofq_linear_ce_bwd(grad.data_ptr(), weight.data_ptr(), _p(bias), kept.data_ptr(), T, D, V, b16,
+                                 int(bias is not None and bias.dtype == torch.bfloat16), smoothing, reduction, _p(dx), _p(dw), _p(db),
+                                 ws.data_ptr(), ws.numel(), _stream()),
              "ofq_linear_ce_bwd")
     return dx, dw, db
 

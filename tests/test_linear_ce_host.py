@@ -31,11 +31,16 @@ def test_module_has_the_functions_checks():
 def test_entries_refuse_bad_arguments_on_the_host():
     from ofq_amd import _lib
     lib = _lib.load()
-    assert lib.ofq_linear_ce_kept_bytes(0, 8, 5, 0, 1) == 0 and lib.ofq_linear_ce_fwd_ws_bytes(4, 0, 5, 0) == 0
+    assert lib.ofq_linear_ce_kept_bytes(0, 8, 5, 0, 1, 1) == 0 and lib.ofq_linear_ce_fwd_ws_bytes(4, 0, 5, 0) == 0
     assert lib.ofq_linear_ce_bwd_ws_bytes(4, 8, (1 << 24) + 1, 0, 1, 1) == 0
     # bf16 whose rows are whole chunks is used in place; anything else is packed
-    small, packed = lib.ofq_linear_ce_kept_bytes(64, 64, 1000, 1, 1), lib.ofq_linear_ce_kept_bytes(64, 64, 1000, 1, 0)
-    assert packed - small == 1000 * 64 * 2 and lib.ofq_linear_ce_kept_bytes(64, 63, 1000, 1, 1) == packed
+    kept = lambda *a: lib.ofq_linear_ce_kept_bytes(*a, 0)
+    assert kept(64, 64, 1024, 1, 0) - kept(64, 64, 1024, 1, 1) == 1024 * 64 * 2 and kept(64, 63, 1024, 1, 1) == kept(64, 64, 1024, 1, 0)
+    # logits up to 128 MB stay for the backward, more do not
+    with_z = lambda *a: lib.ofq_linear_ce_kept_bytes(*a, 1)
+    assert with_z(64, 256, 1024, 0, 1) - kept(64, 256, 1024, 0, 1) == 64 * 1024 * 4
+    assert with_z(64, 64, 1024, 0, 1) == kept(64, 64, 1024, 0, 1)                # (a product over 64 is sooner done again)
+    assert with_z(4096, 256, 16384, 0, 1) == kept(4096, 256, 16384, 0, 1) and with_z(4096, 256, 8192, 0, 1) > kept(4096, 256, 8192, 0, 1)
     none = [None] * 4
-    assert lib.ofq_linear_ce_fwd(*none, 4, 8, 5, 0, 0, -100, 0.0, 1, None, None, None, 0, None, 0, None) != 0
-    assert lib.ofq_linear_ce_bwd(*[None] * 6, 4, 8, 5, 0, 0, -100, 0.0, 1, None, None, None, None, 0, None) != 0
+    assert lib.ofq_linear_ce_fwd(*none, 4, 8, 5, 0, 0, -100, 0.0, 1, 1, None, None, 0, None, 0, None) != 0
+    assert lib.ofq_linear_ce_bwd(*[None] * 4, 4, 8, 5, 0, 0, 0.0, 1, None, None, None, None, 0, None) != 0
