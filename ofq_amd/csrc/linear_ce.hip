@@ -15,6 +15,7 @@
 
 #define CE_AMAX_X 128                    // partial maxima of x and of W
 #define CE_AMAX_W 384
+#define CE_FEW 4                         // rows up to which the gradients of bf16 tensors are one pass over W
 #define CE_PIECE_BYTES (128ll << 20)     // of G: half of the 256 MB last-level cache
 
 struct CeDims {
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
 // shared[0].  G holds (exp(z - lse) - (1 - e)[v = y] - e/V) / unit, times a row's share of the largest gradient: what all rows have in
 // common is multiplied in fp32 at the end.  A target's element, the one that carries a gradient, is then -1 for a class that is not
 // learnt yet, which 16 bits hold exactly; 1/n or 1 - e rounded to bf16 would be one relative error, up to 2^-9, common to all rows, that
-// no sum averages (dW and dx of 7373 rows of bf16: 2.8e-3 from the formula's in 64 bits, against 2.0e-3 so).
+// no sum averages (dW and dx of 4096 rows in bf16: 2.8e-3 from the formula in 64 bits, against 1.8e-3 so).
 struct CeGrad {
   const float* grad; const int* n; const float* shared;
   int reduction;
@@ -640,6 +641,66 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
                  [](int, int, const float (&)[8]) {}, lds);
 }
 
+// Few rows, bf16: both gradients in one pass over W, without the matrix cores.  A thread has eight columns of x and of dx in registers and
+// walks over the vocabulary: reads its 16 bytes of a row of W, adds G times it to dx, writes G times x to dW.  rp rows of W to a
+// workgroup a time, `per` threads to a row (a power of two; blockIdx.y: columns beyond 4096); every row group leaves a partial dx.
+// Bound by memory: one row against 65536 x 2048 reads and writes 268 MB, 94 us (a copy
+// takes 98); the two products take 71 + 88.
+template <int TT>
+__global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __restrict__ w, const unsigned short* __restrict__ G, int64_t ldg,
+                                                     const unsigned short* __restrict__ x, int64_t D, int T, int nv, int per, int acc,
+                                                     float* __restrict__ part, int64_t slot, unsigned short* __restrict__ dw, CeGrad g) {
+  const int r = threadIdx.x / per, rp = 512 / per;
+  const int64_t col = ((int64_t)blockIdx.y * per + threadIdx.x % per) * 8;
+  if (col >= D) return;
+  float xs[TT][8], dx[TT][8];
+  float* mine = part + (blockIdx.x * rp + r) * slot + col;
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      xs[t][e] = g16_f32(x[t * D + col + e]);
+      dx[t][e] = acc && t < T ? mine[t * D + e] : 0.f;
+    }
+  const float f = ce_factor<1>(g);
+  constexpr int U = 4;
+  const int step = gridDim.x * rp;
+  for (int v0 = blockIdx.x * rp + r; v0 < nv; v0 += U * step) {
+    g16_u32x4 q[U];
+    float gv[U][TT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t v = v0 + u * step < nv ? v0 + u * step : v0;
+      q[u] = *reinterpret_cast<const g16_u32x4*>(w + v * D + col);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) gv[u][t] = g16_f32(G[t * ldg + v]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * step >= nv) break;
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float we = __uint_as_float(e & 1 ? q[u][e >> 1] & 0xffff0000u : q[u][e >> 1] << 16);
+        float s = 0.f;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          dx[t][e] = fmaf(gv[u][t], we, dx[t][e]);
+          s = fmaf(gv[u][t], xs[t][e], s);
+        }
+        o[e] = ce_times(s, f);
+      }
+      if (dw) *reinterpret_cast<g16_u32x4*>(dw + (v0 + u * step) * D + col) = g16_bf16x8_of(o);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+    if (t < T) {
+      *reinterpret_cast<float4*>(mine + t * D) = make_float4(dx[t][0], dx[t][1], dx[t][2], dx[t][3]);
+      *reinterpret_cast<float4*>(mine + t * D + 4) = make_float4(dx[t][4], dx[t][5], dx[t][6], dx[t][7]);
+    }
+}
+
 // dx = sum of the split's partials, in order, scaled and typed, and zeros in the rows that do not count; part NULL: those alone
 template <int NP>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, const float* __restrict__ scale,
@@ -662,6 +723,38 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e] * a, b);
     ce_put(dx, out16, t * d.D + c, (int)min((int64_t)8, d.D - c), v);
+  }
+}
+
+// The same where there are few columns and many partials: 32 groups of threads share those of a chunk and meet in LDS
+__global__ __launch_bounds__(256) void ce_dx_few_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, CeRows k, CeGrad g,
+                                                        unsigned short* __restrict__ dx) {
+  __shared__ float sums[32][8][9];
+  const int64_t per = d.Dp / 8, i = blockIdx.x * 8ll + threadIdx.x % 8, t = i / per, c = (i - t * per) * 8;
+  const int l = threadIdx.x % 8, q = threadIdx.x / 8;
+  const int at = t < d.T ? k.pos[t] : -1;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float* p = part + at * d.Dp + c;
+  const int ns = at < 0 ? 0 : split;
+#pragma unroll 8
+  for (int s = q; s < ns; s += 32) {
+    const float4 x = *reinterpret_cast<const float4*>(p + s * slot), y = *reinterpret_cast<const float4*>(p + s * slot + 4);
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[q][l][e] = v[e];
+  for (int half = 16; half > 0; half >>= 1) {
+    __syncthreads();
+    if (q < half) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[q][l][e] = v[e] += sums[q + half][l][e];
+    }
+  }
+  if (q == 0 && t < d.T) {
+    const float f = ce_factor<1>(g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e], f);
+    ce_put(dx, 1, t * d.D + c, 8, v);
   }
 }
 
@@ -790,20 +883,29 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   return 0;
 }
 
-struct CeBwd { int64_t piece, pieces; int split; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
+struct CeBwd { int64_t piece, pieces; int split, few, blocks; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
 static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) {
   CeBwd b;
   b.pieces = ce_pieces(d, &b.piece);
+  // threads to a row of W where both gradients are one pass over it
+  b.few = b.blocks = 0;
+  if (d.np == 1 && !d.pack_w && d.T <= CE_FEW)
+    for (b.few = 8; b.few < 512 && b.few * 8 < d.D; b.few *= 2) {}
   // dx has few tiles and a long k: split it until two workgroups to a CU have work, at no less than eight k-steps each
   const int64_t tiles = ceil_div(d.T, 128) * ceil_div(d.D, 128), steps = b.piece / (d.np == 1 ? 64 : 32);
   b.split = tiles >= 384 ? 1 : (int)std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 8));
+  if (b.few) {
+    const int rp = 512 / b.few;
+    b.blocks = (int)std::min<int64_t>(256, ceil_div(b.piece, 4 * rp));
+    b.split = b.blocks * rp;
+  }
   char* p = (char*)base;
   size_t at = 0;
   b.shared = (float*)p; at += 256;
   b.G = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * b.piece * 2);
   b.slot = d.T * d.Dp;
   b.part = b.split > 1 || b.pieces > 1 ? (float*)(p + at) : nullptr;                    // else dx is written by its product
-  if (want_dx && b.part) at += ce_up((size_t)b.split * b.slot * 4);
+  if ((want_dx || b.few) && b.part) at += ce_up((size_t)b.split * b.slot * 4);
   b.db = (float*)(p + at); if (want_db) at += ce_up((size_t)d.tiles_t * b.piece * 4);
   b.bytes = at;
   return b;
@@ -843,7 +945,15 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     a.g = cg; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
     if (int rc = ce_logits<true>(a, nv, T, bf16, nullptr, st)) return rc;
     const int64_t gpl = d.Tp * b.piece;
-    if (dw) {
+    if (b.few && (dx || dw)) {
+      const dim3 g((unsigned)b.blocks, (unsigned)ceil_div(D, b.few * 8));
+      unsigned short* dwp = dw ? (unsigned short*)dw + v0 * D : nullptr;
+#define CE_FEW_ROWS(TT) hipLaunchKernelGGL(ce_few_kernel<TT>, g, dim3(512), 0, st, (const unsigned short*)w + v0 * D, b.G, b.piece, k.x, D, (int)T, (int)nv, b.few, i > 0, b.part, b.slot, dwp, cg)
+      if (T == 1) CE_FEW_ROWS(1); else if (T == 2) CE_FEW_ROWS(2); else CE_FEW_ROWS(4);
+#undef CE_FEW_ROWS
+      OFQ_LAUNCH_CHECK();
+    }
+    if (dw && !b.few) {
       CeOut o = {};
       o.rows = k.rows;
       o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
@@ -852,7 +962,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
       o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = k.scale; o.g = cg;
       if (int rc = ce_grad<true>(o, bf16, st)) return rc;
     }
-    if (dx) {
+    if (dx && !b.few) {
       CeOut o = {};
       o.rows = k.rows;
       o.P = ce_w_op(d, k, w, v0);
@@ -871,8 +981,10 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     }
   }
   if (dx) {
-    const dim3 g((unsigned)std::min<int64_t>(ceil_div(T * (d.Dp / 8), 256), 8192));
-    if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
+    const int64_t chunks = T * (d.Dp / 8);
+    const dim3 g((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 8192));
+    if (b.few) hipLaunchKernelGGL(ce_dx_few_kernel, dim3((unsigned)ceil_div(chunks, 8)), dim3(256), 0, st, b.part, b.slot, b.split, d, k.rows, cg, (unsigned short*)dx);
+    else if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
     else hipLaunchKernelGGL(ce_dx_kernel<2>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
     OFQ_LAUNCH_CHECK();
   }

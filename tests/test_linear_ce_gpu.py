@@ -117,6 +117,30 @@ def test_many_pieces_of_the_vocabulary(dtype):
     check(got, want, dtype, 16.0)
 
 
+@pytest.mark.parametrize("ignored", [False, True])
+@pytest.mark.parametrize("T,D,V", [(1, 64, 2), (1, 4160, 300), (2, 128, 5000), (3, 512, 777), (4, 2048, 1030), (4, 8192, 65), (5, 512, 777)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_rows_of_bf16(T, D, V, ignored, reduction):
+    """Up to four rows take both gradients in one pass over the weights: columns beyond 4096, vocabularies smaller than the grid, rows
+    that do not count."""
+    x, w, b, y = make(T, D, V, "bf16")
+    if ignored and T > 1:
+        y[T // 2] = -100
+    grad = torch.linspace(-1.0, 2.0, T) if reduction == "none" else None
+    zmax = float((x.double() @ w.double().t()).abs().max()) + 2
+    check(call(x, w, b, y, 0.1, reduction, grad), reference(x, w, b, y, 0.1, reduction, grad), "bf16", zmax)
+
+
+def test_few_rows_with_one_gradient_alone():
+    from ofq_amd.functional import linear_cross_entropy
+    x, w, _, y = make(2, 128, 500, "bf16")
+    both = call(x, w, None, y)
+    xs, ws = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dx, = torch.autograd.grad(linear_cross_entropy(xs, ws.detach(), y.cuda()), [xs])
+    dw, = torch.autograd.grad(linear_cross_entropy(xs.detach(), ws, y.cuda()), [ws])
+    assert torch.equal(dx, both[1]) and torch.equal(dw, both[2])
+
+
 def test_gradient_agrees_with_differences():
     """fp32 loss along a direction: central differences of the 64-bit loss against the kernel's gradient."""
     x, w, b, y = make(37, 48, 90, "fp32", ignored=0.2)
