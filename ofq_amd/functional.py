@@ -1366,6 +1366,6 @@ def linear_cross_entropy(input, weight, target, bias=None, ignore_index=-100, la
     if max(target.numel(), weight.shape[0]) > 1 << 24 or weight.shape[1] > 1 << 20:
         raise ValueError("linear_cross_entropy: at most 2^24 rows and classes and 2^20 features")
     if target.numel() == 0:                     # no rows: a sum of nothing (its gradients are zeros), and a mean over nothing
-        total = input.float().sum() + 0.0 * (weight.float().sum() + (0.0 if bias is None else bias.float().sum()))
+        total = input.float().sum() + weight[:0].float().sum() + (0.0 if bias is None else bias[:0].float().sum())
         return total.expand(target.shape) if reduction == "none" else total if reduction == "sum" else total * float("nan")
     return LinearCrossEntropyFn.apply(input, weight, bias, target, int(ignore_index), float(label_smoothing), reduction)

@@ -266,6 +266,8 @@ class FusedMuon(FusedAdamW):
             if group["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
                 raise ValueError("FusedMuon: adjust_lr_fn must be None, 'original' or 'match_rms_adamw' (got %r)"
                                  % (group["adjust_lr_fn"],))
+            if len({id(p) for p in group["params"]}) != len(group["params"]):
+                raise ValueError("FusedMuon: a parameter is in its group twice")
             for p in group["params"]:
                 if p.dim() != 2:
                     raise ValueError("FusedMuon: matrices only in a Muon group (got shape %s); give other parameters a group with "

@@ -172,6 +172,85 @@ def test_ignored_rows_may_hold_anything(dtype, value):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T,live", [(300, 1), (300, 63), (300, 64), (300, 65), (300, 129), (9001, 70)])
+def test_the_rows_that_count_anywhere_among_many(T, live, dtype):
+    """As many rows as end on, in front of and behind a padding step, spread over the batch (and past what one pass of the numbering holds)."""
+    D, V = 256, 130
+    x, w, b, y = make(T, D, V, dtype)
+    keep = torch.zeros(T, dtype=torch.bool)
+    keep[torch.randperm(T, generator=torch.Generator().manual_seed(live))[:live]] = True
+    keep[-1], keep[0] = True, False
+    y[~keep] = -100
+    x[~keep] = math.nan
+    check(call(x, w, b, y, 0.1), reference(x, w, b, y, 0.1), dtype, 32.0)
+    g = torch.rand(T, generator=torch.Generator().manual_seed(1)) - 0.5
+    got = call(x, w, b, y, 0.0, "none", g)
+    check(got, reference(x, w, b, y, 0.0, "none", g), dtype, 32.0)
+    assert not bool(got[0].detach().cpu()[~keep].any()) and not bool(got[1].cpu()[~keep].any())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T,D,V", [(512, 512, 33000), (300, 320, 9100), (1025, 192, 4100)])
+def test_logits_that_stay_for_the_backward(T, D, V, dtype):
+    """Every tile form a kept grid has, with rests in both directions; without a backward pass nothing is kept and the loss is the same."""
+    from ofq_amd.functional import linear_cross_entropy
+    x, w, b, y = make(T, D, V, dtype, ignored=0.1)
+    got = call(x, w, b, y, 0.1)
+    check(got, reference(x, w, b, y, 0.1), dtype, 32.0)
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x.cuda(), w.cuda(), y.cuda(), bias=b.cuda(), label_smoothing=0.1), got[0].detach())
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_rows_at_all(reduction):
+    x, w, b, y = make(4, 64, 50, "fp32")
+    got = call(x[:0], w, b, y[:0], 0.0, reduction, torch.ones(0) if reduction == "none" else None)
+    assert got[0].shape == ((0,) if reduction == "none" else ())
+    assert math.isnan(float(got[0])) if reduction == "mean" else not bool(got[0].any())
+    if reduction != "mean":
+        assert not any(bool(g.any()) for g in got[1:])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_an_overflowed_gradient_stays_in_the_rows_that_count(dtype):
+    """A loss scale that overflowed sends Inf in: rows that do not count still get zeros, the others nothing finite that is not zero."""
+    x, w, b, y = make(70, 64, 90, dtype, ignored=0.3)
+    dead = y == -100
+    for reduction, grad in (("mean", math.inf), ("none", torch.full((70,), math.inf))):
+        dx = call(x, w, b, y, 0.0, reduction, grad)[1].float().cpu()
+        assert not bool(dx[dead].any()) and not bool(torch.isfinite(dx[~dead]).any())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_a_graph_replayed_with_other_numbers_of_rows(dtype):
+    """The number of rows that count is read on the device: a captured pass follows it from all rows to none."""
+    from ofq_amd.functional import linear_cross_entropy
+    x, w, _, y = make(260, 256, 300, dtype)
+    xs, ws, ys = x.cuda().requires_grad_(), w.cuda().requires_grad_(), y.cuda()
+
+    def step():
+        loss = linear_cross_entropy(xs, ws, ys, reduction="sum")
+        return (loss.detach(),) + torch.autograd.grad(loss, (xs, ws))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for live in (260, 100, 0, 1, 200):
+        t = y.clone()
+        t[live:] = -100
+        ys.copy_(t)
+        graph.replay()
+        eager = call(x, w, None, t, 0.0, "sum")
+        torch.cuda.synchronize()
+        for a, c in zip(out, eager):
+            assert torch.equal(a, c.detach())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_no_live_row(dtype):
     x, w, b, y = make(5, 64, 10, dtype)
     y[:] = -100

@@ -317,3 +317,69 @@ def test_a_training_step_with_both_ends():
     ga, gb = torch.autograd.grad(fused, params), torch.autograd.grad(plain, params)
     scale = max(float(g.norm()) for g in gb)
     assert all(float((a - b).norm()) <= 1e-4 * scale for a, b in zip(ga, gb))
+
+
+def test_a_captured_training_step_under_both_rules():
+    """engine.GraphedTrainStep with the optimiser of opt="muon", the learning rate changing: losses, parameters and momentum are the
+    eager steps', bit for bit."""
+    import copy
+    from functools import partial
+    from types import SimpleNamespace
+
+    import torch.nn as nn
+    from ofq_amd import engine
+    from ofq_amd.deit import DistilledVisionTransformer
+    torch.manual_seed(0)
+    base = DistilledVisionTransformer(img_size=224, patch_size=16, embed_dim=64, depth=2, num_heads=2, mlp_ratio=4, qkv_bias=True,
+                                      num_classes=50, norm_layer=partial(nn.LayerNorm, eps=1e-6), act_layer=nn.GELU)
+    args = SimpleNamespace(qmodules=engine.default_qmodules(2), wq_mode="statsq", wq_enable=True, wq_bitw=4, aq_enable=True, aq_mode="lsq",
+                           aq_bitw=4, wq_per_channel=True, aq_per_channel=True, model_type="deit", pretrained_initialized=True,
+                           qk_reparam=True, qk_reparam_type=0)
+    base = engine.get_qat_model(base, args).cuda()
+    g = torch.Generator().manual_seed(1)
+    batches = [(torch.randn(4, 3, 224, 224, generator=g).cuda(), torch.randint(0, 50, (4,), generator=g).cuda(),
+                torch.randn(4, 50, generator=g).cuda()) for _ in range(2)]
+    engine.setup_alpha(base, batches[0][0])
+    from ofq_amd.quantization.utils import KDLossSoftandHard
+    results = []
+    for graphed in (False, True):
+        model = copy.deepcopy(base).train()
+        opt = engine.make_optimizer(model, lr=1e-3, opt="muon")
+        loss_fn = KDLossSoftandHard()
+        gs = engine.GraphedTrainStep(model, opt, loss_fn, warmup=2) if graphed else None
+        losses = []
+        for i in range(6):
+            for group in opt.param_groups:
+                group["lr"] = 1e-3 * (1 - 0.1 * i)
+            img, y, soft = batches[i % 2]
+            loss = gs(img, y, soft) if graphed else engine.train_step(model, opt, img, y, soft, loss_fn)
+            losses.append(float(loss.detach()))
+        state = [opt.state[p].get("momentum_buffer") for p in model.parameters()]
+        results.append((losses, [p.detach().clone() for p in model.parameters()], state))
+    (la, pa, sa), (lb, pb, sb) = results
+    assert la == lb
+    assert all(torch.equal(a, b) for a, b in zip(pa, pb))
+    assert sum(a is not None for a in sa) > 0
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(sa, sb))
+
+
+def test_train_command_with_muon(tmp_path):
+    """train.py --opt muon: two epochs of two steps, and a run resumed after the first goes on with the same losses."""
+    import contextlib
+    import io
+
+    from ofq_amd import train_cli
+    common = ["--model", "deit_tiny_distilled_patch16_224", "--batch-size", "4", "--steps-per-epoch", "2", "--val-steps", "1",
+              "--lr", "5e-4", "--weight-decay", "0.05", "--aq-enable", "--aq-mode", "lsq", "--aq-per-channel", "--aq_clip_learnable",
+              "--aq-bitw", "3", "--wq-enable", "--wq-per-channel", "--wq-bitw", "3", "--wq-mode", "statsq", "--model_type", "deit",
+              "--quantized", "--qk_reparam", "--qk_reparam_type", "0", "--log-interval", "1", "--warmup-epochs", "0", "--opt", "muon"]
+
+    def run(extra):
+        buf = io.StringIO()
+        with contextlib.redirect_stdout(buf):
+            train_cli.main(common + extra)
+        return [float(l.split("Loss:")[1].split()[0]) for l in buf.getvalue().splitlines() if l.startswith("Train:")]
+    full = run(["--epochs", "2", "--output", str(tmp_path / "full")])
+    run(["--epochs", "1", "--output", str(tmp_path / "half")])
+    rest = run(["--epochs", "2", "--resume", str(tmp_path / "half" / "last.pth.tar"), "--output", str(tmp_path / "res")])
+    assert len(full) == 4 and rest == pytest.approx(full[2:], rel=1e-6)

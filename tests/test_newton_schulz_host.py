@@ -45,6 +45,9 @@ def test_muon_groups_hold_matrices():
     assert len(opt.param_groups) == 1
     p = torch.nn.Parameter(torch.zeros(2, 2))
     opt.add_param_group({"params": [p]})
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning):
+        q = torch.nn.Parameter(torch.zeros(2, 2))
+        opt.add_param_group({"params": [q, q]})
     opt.set_frozen(v, torch.ones(3))
     with pytest.raises(RuntimeError, match="freeze"):
         opt.set_frozen(p, torch.ones(2, 2))
