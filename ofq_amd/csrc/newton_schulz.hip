@@ -55,7 +55,7 @@ __device__ __forceinline__ float ns_load(const void* g, int64_t i) {
 }
 
 // m <- m + (1 - mu)(g - m), and the sum of squares of u = m or (Nesterov) m - (1 - mu)(m - g); doubles, so that neither tiny nor huge
-// gradients leave the range of their squares.  HBM-bound: reads g and m, writes m.
+// gradients leave the range of their squares.  HBM-bound: reads g and m, writes m: 25 million elements in 55 us, 5.4 TB/s.
 template <bool BF16>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsRec* __restrict__ t, int n, NsStep st, const unsigned* __restrict__ guard,
                                                       double* __restrict__ parts) {
@@ -117,7 +117,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsRec* __restrict__ 
   if (threadIdx.x == 0) parts[r.part + blockIdx.x - r.p0] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// X planes = u / max(|u|_F, eps) * 2^10, transposed where rows > columns, zero padded to [mp][np].  64 x 64 blocks through LDS.
+// X planes = u / max(|u|_F, eps) * 2^10, transposed where rows > columns, zero padded to [mp][np].  64 x 64 blocks through LDS.  25 million
+// elements in 67 us, 3 TB/s: scalar loads, as either side may be the transposed one.
 template <bool BF16>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ t, int n, NsStep st, float eps,
                                                       const double* __restrict__ parts, _Float16* __restrict__ ws) {
@@ -170,6 +171,10 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ 
 // One tile (tr >= tc) of a symmetric matrix: A = X X^T (SQUARE false: k along X's rows) or B = b A + c A A (k along A's).
 // Matrices of unlike lengths in one launch of X X^T wait for the longest tiles: cut along k into pieces (added up by the last to
 // arrive) they were no faster, the pieces' way through memory costs what the balance gains.
+// Matrix cores: twelve of 1024 x 1024 / 4096 113 us (X X^T, 690 TFLOP/s of plane products: its longest tiles are 128 k-steps) and 75 us
+// (squares, 515: 432 tiles for 512 places); thirty of 384 / 1536 36 and 23 us, of which a tile's start and end are about half.
+// Taking short matrices a product behind the long ones, so that one launch mixes short and long tiles, gained 2 % there and lost 20 % on
+// the larger ones.
 template <int CFG, bool SQUARE>
 __global__ __launch_bounds__(g16_nt(CFG)) void ns_sym_kernel(const NsRec* __restrict__ t, int n, float fb, float fc, int odd, int run,
                                                              _Float16* __restrict__ ws) {
@@ -214,7 +219,8 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ns_sym_kernel(const NsRec* __rest
   else g16_store_tile<2, CFG, true>(value, direct, mirror, lds);
 }
 
-// X <- a X + B X: r runs along the columns of X, c along its rows
+// X <- a X + B X: r runs along the columns of X, c along its rows.  Matrix cores: twelve of 1024 x 1024 / 4096 181 us, 860 TFLOP/s of plane
+// products; six of 2048 x 2048 / 8192 640 us, 970.
 template <int CFG>
 __global__ __launch_bounds__(g16_nt(CFG)) void ns_update_kernel(const NsRec* __restrict__ t, int n, float fa, int odd, _Float16* __restrict__ ws) {
   using C = G16<2, CFG>;
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ns_update_kernel(const NsRec* __r
 }
 
 // out = O (the update's own type), or the parameter p <- p decay - lr wscale O; hyper: {lr, decay} from device memory (a captured
-// step), guard: the step's guard word (see adamw.hip)
+// step), guard: the step's guard word (see adamw.hip).  HBM-bound: 25 million elements in 64 us, 4.6 TB/s.
 template <bool BF16>
 __global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__ t, int n, NsStep st, const float* __restrict__ hyper,
                                                        const unsigned* __restrict__ guard, int odd, const _Float16* __restrict__ ws) {
