@@ -559,7 +559,7 @@ int ofq_input_pipeline_u8(const uint8_t* in, float* out, int64_t B, int64_t C, i
  *  with target == ignore_index lose nothing, receive no gradient, whatever x holds there, and cost nothing; a target outside the
  *  vocabulary makes its loss NaN.  reduction: 0 none (loss [T]), 1 mean over the other rows (NaN without any), 2 sum; loss fp32.
  *  kept: what the backward needs beside its arguments (ofq_linear_ce_kept_bytes; w_aligned = w is a multiple of 16 bytes; backward = 0:
- *  none is to come), ws: scratch; both 256-byte aligned device memory of the caller.
+ *  none is to come; the backward pass refuses another size than its own), ws: scratch; both 256-byte aligned device memory of the caller.
  *  bwd: grad = the incoming gradient (one float; reduction 0: [T]); dx [T][D], dw [V][D] in the tensors' type, db [V] in the
  *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.
  *  T <= 2^24, V <= 2^24, D <= 2^20. */
@@ -569,8 +569,8 @@ size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int
 int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
                       int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, int backward, float* loss,
                       void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, ofq_stream_t stream);
-int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, int64_t T, int64_t D, int64_t V,
-                      int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream);
+int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, size_t kept_bytes, int64_t T, int64_t D,
+                      int64_t V, int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream);
 
 /* ---- Newton-Schulz orthogonalisation of many matrices, and the optimiser step around it (csrc/newton_schulz.hip)
  *  tensors: HOST array of n records of ofq_newton_schulz_entry_bytes() bytes

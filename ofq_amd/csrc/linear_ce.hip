@@ -18,6 +18,11 @@
 #define CE_FEW 4                         // rows up to which the gradients of bf16 tensors are one pass over W
 #define CE_PIECE_BYTES (128ll << 20)     // of G: half of the 256 MB last-level cache
 
+static int ce_form(int64_t R, int64_t C, int split) {
+  auto tiles = [&](int t) { return ceil_div(R, t) * ceil_div(C, t) * split; };
+  return g16_form(tiles(64), tiles(128), tiles(256));
+}
+
 struct CeDims {
   int64_t T, D, V, Tp, Dp, Vp, tiles_v, tiles_t;
   int np;
@@ -27,7 +32,8 @@ static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, Ce
   if (T <= 0 || D <= 0 || V <= 0 || T > (1 << 24) || D > (1 << 20) || V > (1 << 24)) return false;
   auto pad = [](int64_t v) { return (v + G16_PAD - 1) / G16_PAD * G16_PAD; };
   d->T = T; d->D = D; d->V = V; d->Tp = pad(T); d->Dp = pad(D); d->Vp = pad(V);
-  d->tiles_v = ceil_div(V, 64); d->tiles_t = ceil_div(T, 64);        // at most
+  d->tiles_v = ceil_div(V, g16_t(ce_form(V, T, 1)));                 // of the forward pass
+  d->tiles_t = ceil_div(T, 64);                                      // at most
   d->np = bf16 ? 1 : 2;
   d->pack_w = !bf16 || d->Dp != D || !w_aligned;
   return true;
@@ -42,10 +48,6 @@ static int64_t ce_pieces(const CeDims& d, int64_t* piece) {
   const int64_t round = std::max<int64_t>(256 / ceil_div(d.D, 256), 1) * 256;
   *piece = vp <= most ? vp : most >= round ? most / round * round : most;
   return ceil_div(vp, *piece);
-}
-static int ce_form(int64_t R, int64_t C, int split) {
-  auto tiles = [&](int t) { return ceil_div(R, t) * ceil_div(C, t) * split; };
-  return g16_form(tiles(64), tiles(128), tiles(256));
 }
 // Logits of a single piece are kept (its G takes as much again for a while) where the product takes longer than their way to memory and
 // back; else they are computed a second time.  Kept / not, us, 2 directions: bf16, 64 x 65536, D 2048: 267 / 306; 509 x 21841, D 768:
@@ -858,8 +860,7 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   const CeKept k = ce_kept(kept, d, backward != 0);
   const CeFwdWs f = ce_fwd_ws(ws, d);
   if (kept_bytes < k.bytes || ws_bytes < f.bytes) return OFQ_ENOWS;
-  const int64_t tiles = d.tiles_v * d.tiles_t;
-  if (tiles >= (1ll << 31)) return OFQ_EINVAL;
+  if (ceil_div(V, 64) * d.tiles_t >= (1ll << 31)) return OFQ_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   float* rows_out = reduction == 0 ? loss : nullptr;
   if (bf16) hipLaunchKernelGGL(ce_number_kernel, dim3(1), dim3(1024), 0, st, target, ignore_index, T, (int)V, k.rows, rows_out);
@@ -929,13 +930,14 @@ extern "C" size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, in
 }
 
 // grad: the incoming gradient, one float or (reduction 0) [T]; kept as a forward pass with backward != 0 left it; dx / dw / db: any may be NULL
-extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, int64_t T, int64_t D, int64_t V,
-                                 int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream) {
+extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, size_t kept_bytes, int64_t T, int64_t D,
+                                 int64_t V, int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream) {
   CeDims d;
   if (!grad || !w || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
       !ce_dims(T, D, V, bf16, ce_w_aligned(w), &d) || ((uintptr_t)kept & 255) || ((uintptr_t)ws & 255))
     return OFQ_EINVAL;
   const CeKept k = ce_kept((void*)kept, d, true);
+  if (kept_bytes != k.bytes) return OFQ_EINVAL;          // another size, or weights that moved to another alignment since
   const CeBwd b = ce_bwd_ws(ws, d, dx != nullptr, db != nullptr);
   if (ws_bytes < b.bytes) return OFQ_ENOWS;
   hipStream_t st = (hipStream_t)stream;

@@ -1329,6 +1329,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         w, b, kept = ctx.saved_tensors
+        w = w.contiguous()                     # (as it was saved, unless a saved-tensor hook put another in its place)
         shape, T, smoothing, red = ctx.args
         need = ctx.needs_input_grad
         with ops.on_device(w.device):

@@ -383,6 +383,24 @@ def test_weight_changed_between_forward_and_backward_is_refused():
         loss.backward()
 
 
+def test_weights_that_come_back_at_another_alignment():
+    """A saved-tensor hook may hand the backward a copy: at another alignment than the forward's (which had packed it) it is refused; one
+    that went to the host and back is as good as the original."""
+    from ofq_amd.functional import linear_cross_entropy
+    x, w, _, y = make(40, 64, 300, "bf16")
+    xs, ys = x.cuda().requires_grad_(), y.cuda()
+    odd = torch.empty(300 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(300, 64).copy_(w.cuda()).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.clone()):
+        loss = linear_cross_entropy(xs, odd, ys)
+        with pytest.raises(RuntimeError, match="ofq_linear_ce_bwd"):
+            loss.backward()
+    want = call(x, w, None, y)
+    ws = w.cuda().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        dx, dw = torch.autograd.grad(linear_cross_entropy(xs, ws, ys), [xs, ws])
+    assert torch.equal(dx, want[1]) and torch.equal(dw, want[2])
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_captured_forward_and_backward_replayed(dtype):
     """The graph replayed with other inputs in its static buffers, with eager work and synchronisations between the replays."""

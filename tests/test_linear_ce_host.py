@@ -43,4 +43,4 @@ def test_entries_refuse_bad_arguments_on_the_host():
     assert with_z(4096, 256, 16384, 0, 1) == kept(4096, 256, 16384, 0, 1) and with_z(4096, 256, 8192, 0, 1) > kept(4096, 256, 8192, 0, 1)
     none = [None] * 4
     assert lib.ofq_linear_ce_fwd(*none, 4, 8, 5, 0, 0, -100, 0.0, 1, 1, None, None, 0, None, 0, None) != 0
-    assert lib.ofq_linear_ce_bwd(*[None] * 4, 4, 8, 5, 0, 0, 0.0, 1, None, None, None, None, 0, None) != 0
+    assert lib.ofq_linear_ce_bwd(*[None] * 4, 0, 4, 8, 5, 0, 0, 0.0, 1, None, None, None, None, 0, None) != 0
