@@ -584,6 +584,8 @@ struct CeOut {
   int acc;
   void* out; int out16; int64_t ldo;       // else the final tensor, typed, times 1 / (scale * G's scale)
   const float* scale; CeGrad g;            // scale: of P
+  const float* cols; int cols_tl;          // dW: the column sums that G's tiles of cols_tl rows left, or NULL; db: their sum
+  void* db; int db16;
 };
 
 // n of eight values (n <= 8) to element `at` of a typed tensor, 16 bytes at a time where aligned
@@ -605,6 +607,24 @@ __device__ __forceinline__ void ce_put(void* out, int out16, int64_t at, int n, 
   }
 }
 
+// one element of the bias gradient: the sums of a column over ce_padded(n) / TL tiles, in order
+template <int NP>
+__device__ __forceinline__ void ce_put_db(const float* __restrict__ cols, int64_t ldg, int TL, int c, const CeGrad& g, void* __restrict__ db, int out16) {
+  float s = 0.f;
+  const int ny = (ce_padded(*g.n) + TL - 1) / TL;
+#pragma unroll 8
+  for (int k = 0; k < ny; ++k) s += cols[k * ldg + c];
+  s = ce_times(s, ce_factor<NP>(g));
+  if (out16) reinterpret_cast<unsigned short*>(db)[c] = g16_bf16(s);
+  else reinterpret_cast<float*>(db)[c] = s;
+}
+// where no dW product takes it along
+template <int NP>
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ cols, int64_t ldg, int TL, int n, CeGrad g, void* __restrict__ db, int out16) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < n) ce_put_db<NP>(cols, ldg, TL, c, g, db, out16);
+}
+
 // dx (QCOL false: P = W [k = v][r = d], Q = G [c = t][k = v]) and dW (QCOL true: P = x [k = t][r = d], Q = G [k = t][c = v]); t: packed rows.
 // A part of a split k has consecutive workgroups of one XCD, so that they take whole rows of W.  Bound by the matrix cores: 4096 x 16384 of
 // 4096 bf16 dx 475 and dW 490 us (1100 and 1070 TFLOP/s); fp32 509 x 21841 of 768 61 and 80 us (840 and 640 of the three products: dW has
@@ -616,7 +636,17 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
   const int id = g16_xcd(blockIdx.x, gridDim.x, gridDim.x), tiles = p.tiles_r * p.tiles_c, sp = id / tiles, n = *p.rows.n;
   int tr, tc;
   g16_group(id - sp * tiles, p.tiles_r, p.tiles_c, tr, tc);
-  if (!QCOL && tc * C::T >= n) return;
+  if constexpr (!QCOL) {
+    if (!p.part) {                                   // dx itself: this tile's share of the rows that do not count
+      constexpr int PER = C::T / 8;
+      const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int i = threadIdx.x; i < C::T * PER; i += g16_nt(CFG)) {
+        const int t = tc * C::T + i / PER, col = tr * C::T + i % PER * 8;
+        if (t < p.C && col < p.R && p.rows.pos[t] < 0) ce_put(p.out, p.out16, t * p.ldo + col, p.R - col, zero);
+      }
+    }
+    if (tc * C::T >= n) return;
+  }
   constexpr int BK = C::BK;
   const int nk = (QCOL ? ce_padded(n) : p.K) / BK, per = (nk + p.split - 1) / p.split;
   const int kb = min(sp * per, nk), ke = min(kb + per, nk);
@@ -651,6 +681,10 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
                    }
                  },
                  [](int, int, const float (&)[8]) {}, lds);
+  if constexpr (QCOL) {
+    const int c = tc * C::T + threadIdx.x;
+    if (p.cols && tr == 0 && threadIdx.x < C::T && c < p.C) ce_put_db<NP>(p.cols, p.Q.ld, p.cols_tl, c, p.g, p.db, p.db16);
+  }
 }
 
 // Few rows, bf16: both gradients in one pass over W, without the matrix cores.  A thread has eight columns of x and of dx in registers and
@@ -713,7 +747,7 @@ __global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __res
     }
 }
 
-// dx = sum of the split's partials, in order, scaled and typed, and zeros in the rows that do not count; part NULL: those alone
+// dx = sum of the split's partials, in order, scaled and typed, and zeros in the rows that do not count
 template <int NP>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, const float* __restrict__ scale,
                                                     CeRows k, CeGrad g, void* __restrict__ dx, int out16) {
@@ -724,7 +758,6 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
     if (c >= d.D) continue;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const int at = k.pos[t];
-    if (at >= 0 && !part) continue;
     const float* p = part + at * d.Dp + c;
     const int ns = at < 0 ? 0 : split;
 #pragma unroll 8
@@ -768,21 +801,6 @@ __global__ __launch_bounds__(256) void ce_dx_few_kernel(const float* __restrict_
     for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e], f);
     ce_put(dx, 1, t * d.D + c, 8, v);
   }
-}
-
-// the bias gradient from the sums of columns of ce_padded(n) / TL tiles, in order
-template <int NP>
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int64_t ldg, int TL, int n, CeGrad g, void* __restrict__ db,
-                                                    int out16, int64_t at) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float s = 0.f;
-  const int ny = (ce_padded(*g.n) + TL - 1) / TL;
-#pragma unroll 8
-  for (int k = 0; k < ny; ++k) s += part[k * ldg + c];
-  s = ce_times(s, ce_factor<NP>(g));
-  if (out16) reinterpret_cast<unsigned short*>(db)[at + c] = g16_bf16(s);
-  else reinterpret_cast<float*>(db)[at + c] = s;
 }
 
 static int ce_w_aligned(const void* w) { return ((uintptr_t)w & 15) == 0; }
@@ -905,6 +923,7 @@ static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) 
   // dx has few tiles and a long k: split it so that two workgroups to a CU have work, and none waits for a place (24 tiles, k 21888, two
   // planes: 528 workgroups 86 us, 504 61), at no less than eight k-steps each
   const int64_t tiles = ceil_div(d.T, 128) * ceil_div(d.D, 128), steps = b.piece / (d.np == 1 ? 64 : 32);
+  // (32 steps of the fp32 head of 1000 classes: 25 us at once, three parts 8 and 5 for the launch that joins them)
   b.split = (int)std::max<int64_t>(1, std::min(512 / tiles, steps / 8));
   if (b.few) {
     const int rp = 512 / b.few;
@@ -931,7 +950,8 @@ extern "C" size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, in
 
 // grad: the incoming gradient, one float or (reduction 0) [T]; kept as a forward pass with backward != 0 left it; dx / dw / db: any may be NULL
 extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* bias, const void* kept, size_t kept_bytes, int64_t T, int64_t D,
-                                 int64_t V, int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, ofq_stream_t stream) {
+                                 int64_t V, int bf16, int bias16, float smoothing, int reduction, void* dx, void* dw, void* db, void* ws,
+                                 size_t ws_bytes, ofq_stream_t stream) {
   CeDims d;
   if (!grad || !w || !kept || !ws || reduction < 0 || reduction > 2 || !(smoothing >= 0.f && smoothing <= 1.f) ||
       !ce_dims(T, D, V, bf16, ce_w_aligned(w), &d) || ((uintptr_t)kept & 255) || ((uintptr_t)ws & 255))
@@ -973,6 +993,10 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.R = (int)D; o.C = (int)nv; o.K = (int)d.Tp; o.split = 1;
       o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = k.scale; o.g = cg;
+      if (db) {
+        o.cols = b.db; o.cols_tl = g16_t(ce_form(nv, T, 1));
+        o.db = (char*)db + v0 * (bias16 ? 2 : 4); o.db16 = bias16;
+      }
       if (int rc = ce_grad<true>(o, bf16, st)) return rc;
     }
     if (dx && !b.few) {
@@ -985,15 +1009,16 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
       else { o.R = (int)D; o.out = dx; o.out16 = bf16; o.ldo = D; }
       if (int rc = ce_grad<false>(o, bf16, st)) return rc;
     }
-    if (db) {
+    if (db && (!dw || b.few)) {
       const dim3 g((unsigned)ceil_div(nv, 256));
       const int tl = g16_t(ce_form(nv, T, 1));
-      if (bf16) hipLaunchKernelGGL(ce_db_kernel<1>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, db, bias16, v0);
-      else hipLaunchKernelGGL(ce_db_kernel<2>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, db, bias16, v0);
+      char* to = (char*)db + v0 * (bias16 ? 2 : 4);
+      if (bf16) hipLaunchKernelGGL(ce_db_kernel<1>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, to, bias16);
+      else hipLaunchKernelGGL(ce_db_kernel<2>, g, dim3(256), 0, st, b.db, b.piece, tl, (int)nv, cg, to, bias16);
       OFQ_LAUNCH_CHECK();
     }
   }
-  if (dx) {
+  if (dx && b.part) {
     const int64_t chunks = T * (d.Dp / 8);
     const dim3 g((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 8192));
     if (b.few) hipLaunchKernelGGL(ce_dx_few_kernel, dim3((unsigned)ceil_div(chunks, 8)), dim3(256), 0, st, b.part, b.slot, b.split, d, k.rows, cg, (unsigned short*)dx);
