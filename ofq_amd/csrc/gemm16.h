@@ -163,9 +163,9 @@ __device__ __forceinline__ void g16_read(G16Frags<NP, CFG>& f, const G16Lds& s, 
   else f.b[q][i - RB] = g16_frag<NP, CFG, QCOL>(s.q[buf], q, wc * CB + i - RB, ks, lane);
 }
 // MFMA number n of RB CB (NP = 1) or 3 RB CB (hi hi, hi lo, lo hi).  Inside an MFMA products are cut off some bits below the accumulator's
-// last place (its final rounding is to nearest).  Accumulators of 32 k each, added up with v_add_f32, halved the error of the sums but
-// took 9 % of the time; as it is the Newton-Schulz chain is 1.1e-6 to 2.9e-6 off where fp32 products are 1.5e-6 to 3.9e-6 off, so
-// that is left out.
+// last place (its final rounding is to nearest).  Accumulators of 32 to 128 k each, added up with v_add_f32, halve the error of long
+// sums.  TINY has them: its time is a latency.  In the other forms they took 9 %; there the Newton-Schulz chain is 1.1e-6 to 2.9e-6 off where
+// fp32 products are 1.5e-6 to 3.9e-6 off, so they are left out.
 template <int NP, int CFG, int N>
 __device__ __forceinline__ void g16_mma(G16Acc<NP, CFG>& acc, const G16Frags<NP, CFG>& f) {
   constexpr int RB = G16<NP, CFG>::RB, CB = G16<NP, CFG>::CB, m = N / (RB * CB), i = N / CB % RB, j = N % CB, pa = m == 2, pb = m == 1;
@@ -236,12 +236,26 @@ __device__ __forceinline__ void g16_tile(G16Acc<NP, CFG>& acc, const G16Op& P, c
     constexpr int FIRST = NL / SPREAD;                                         // loads of a phase
     static_assert(SPREAD <= KS && NL % SPREAD == 0, "the loads are out before the next barrier");
     G16Frags<NP, CFG> f[2];
+    // TINY: accumulators of D stages each
+    constexpr bool PART = CFG == G16_TINY;
+    G16Acc<NP, CFG> part;
+    auto& sum = *[&] { if constexpr (PART) return &part; else return &acc; }();
+    auto flush = [&](bool add) {
+#pragma unroll
+      for (int i = 0; i < C::RB; ++i)
+#pragma unroll
+        for (int j = 0; j < C::CB; ++j) {
+          if (add) acc[i][j] += part[i][j];
+          part[i][j] = g16_f32x16{};
+        }
+    };
+    if constexpr (PART) flush(false);
     // The MFMAs of phase ks, and behind them the reads of the next one (rks of buffer rb) and loads [L0, L0 + N) of stage lt into buffer lb
     auto phase = [&](int ks, int rb, int rks, int lb, int lt, auto l0_, auto n_) {
       constexpr int L0 = l0_(), N = n_();
       g16_for<NM>([&](auto m_) {
         constexpr int m = m_();
-        g16_mma<NP, CFG, m>(acc, f[ks & 1]);
+        g16_mma<NP, CFG, m>(sum, f[ks & 1]);
         constexpr int ra = m * NR / NM, re = (m + 1) * NR / NM, la = m * N / NM, le = (m + 1) * N / NM;
         g16_for<re - ra>([&](auto d) { g16_read<NP, CFG, PCOL, QCOL, ra + d()>(f[(ks + 1) & 1], s, rb, rks, wr, wc, lane); });
         g16_for<le - la>([&](auto d) { load1(lb, L0 + la + d(), lt); });
@@ -261,6 +275,7 @@ __device__ __forceinline__ void g16_tile(G16Acc<NP, CFG>& acc, const G16Op& P, c
       g16_for<D>([&](auto u_) {
         constexpr int u = u_();
         if (done) return;
+        if constexpr (PART && u == 0) flush(true);
         // all phases of stage t + u but the last, with what is left of the loads of the stage before
         g16_for<KS - 1>([&](auto ks_) {
           constexpr int ks = ks_();
@@ -273,7 +288,8 @@ __device__ __forceinline__ void g16_tile(G16Acc<NP, CFG>& acc, const G16Op& P, c
       });
       if (done) break;
     }
-    g16_for<NM>([&](auto n) { g16_mma<NP, CFG, n()>(acc, f[(KS - 1) & 1]); });
+    g16_for<NM>([&](auto n) { g16_mma<NP, CFG, n()>(sum, f[(KS - 1) & 1]); });
+    if constexpr (PART) flush(true);
     g16_barrier<0>();                                    // the repeated loads land before the buffers serve the epilogue
   }
 }

@@ -5,8 +5,8 @@
 //             planes; dx += G W and dW = G^T x of that piece; db = column sums of G
 // The tile computes z transposed (r = vocabulary, c = token): a lane holds 32 logits of one token, so the softmax statistics
 // need one exchange between lane halves instead of five steps for each of 32 rows.
-// bf16 tensors go to the matrix cores as they are, G is rounded to bf16 (2^-9 relative, as the gradients themselves are; what all its
-// rows have in common is left out of it, CeGrad).  fp32 tensors are split into two fp16 planes scaled by a power of two taken from the
+// bf16 tensors go to the matrix cores as they are, G is rounded to bf16 (off by up to 2^-8 relative, as the gradients themselves are; what
+// all its rows have in common is left out of it, CeGrad; up to 64 rows it has two planes, ce_dims).  fp32 tensors are split into two fp16 planes scaled by a power of two taken from the
 // tensor's largest element (gemm16.h); G likewise.  Statistics, sums and partial gradients are fp32.
 // Rows whose target is ignore_index are left out of all of it (CeRows): they cost nothing and what they hold (NaN, Inf) reaches nothing.
 // Bound by the matrix cores: 8 n V D operations for n rows that count, of which the recomputation is 2 n V D (6 where the logits are kept,
@@ -15,6 +15,7 @@
 
 #define CE_AMAX_X 128                    // partial maxima of x and of W
 #define CE_AMAX_W 384
+#define CE_FINE G16_PAD                  // rows up to which G of bf16 tensors has two planes
 #define CE_FEW 4                         // rows up to which the gradients of bf16 tensors are one pass over W
 #define CE_PIECE_BYTES (128ll << 20)     // of G: half of the 256 MB last-level cache
 
@@ -25,7 +26,7 @@ static int ce_form(int64_t R, int64_t C, int split) {
 
 struct CeDims {
   int64_t T, D, V, Tp, Dp, Vp, tiles_v, tiles_t;
-  int np;
+  int np, gp;                // planes of the operands, of G
   bool pack_w;
 };
 static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, CeDims* d) {
@@ -35,6 +36,9 @@ static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, Ce
   d->tiles_v = ceil_div(V, g16_t(ce_form(V, T, 1)));                 // of the forward pass
   d->tiles_t = ceil_div(T, 64);                                      // at most
   d->np = bf16 ? 1 : 2;
+  // G of few bf16 rows is held to 16 bits: where one row's rounding is not averaged with others' it showed in the whole gradient (two rows of
+  // three classes: dx 2.3e-3 off, the rounding of the outputs alone 1.6e-3), and their time is W's way from memory.
+  d->gp = bf16 && T > CE_FINE ? 1 : 2;
   d->pack_w = !bf16 || d->Dp != D || !w_aligned;
   return true;
 }
@@ -44,7 +48,7 @@ static size_t ce_up(size_t b) { return (b + 255) & ~(size_t)255; }
 // CUs in dW (and, for as many rows, in G), the last one what is left.  100000 columns of 4096, 4096 rows: seven of 14336 are 3.5 rounds
 // each, 12.9 ms; six of 16384 and a rest 12.0.
 static int64_t ce_pieces(const CeDims& d, int64_t* piece) {
-  const int64_t vp = ceil_div(d.V, 128) * 128, most = std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.np) / 128 * 128, 128);
+  const int64_t vp = ceil_div(d.V, 128) * 128, most = std::max<int64_t>(CE_PIECE_BYTES / (d.Tp * 2 * d.gp) / 128 * 128, 128);
   const int64_t round = std::max<int64_t>(256 / ceil_div(d.D, 256), 1) * 256;
   *piece = vp <= most ? vp : most >= round ? most / round * round : most;
   return ceil_div(vp, *piece);
@@ -274,6 +278,7 @@ struct CeLogits {
   float eps;
   float2* part; float* zsum; float* zy;              // forward: [tiles_v][Tp] (max, sum exp), sum of logits; the target's logit
   CeGrad g; unsigned short* G; int64_t ldg;          // backward
+  int gp;                                            // G's planes
   float* db;                                         // column sums of G's tiles [tiles_c][ldg], or NULL
 };
 
@@ -453,7 +458,14 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
           if (row >= p.Tp || col >= p.ldg) return;
           unsigned short* dst = p.G + row * p.ldg + col;
           if constexpr (NP == 1) {
-            *reinterpret_cast<g16_u32x4*>(dst) = g16_bf16x8_of(v);
+            const g16_u32x4 hi = g16_bf16x8_of(v);
+            *reinterpret_cast<g16_u32x4*>(dst) = hi;
+            if (p.gp == 2) {
+              float rest[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) rest[e] = v[e] - __uint_as_float(e & 1 ? hi[e >> 1] & 0xffff0000u : hi[e >> 1] << 16);
+              *reinterpret_cast<g16_u32x4*>(dst + (int64_t)p.Tp * p.ldg) = g16_bf16x8_of(rest);
+            }
           } else {
             g16_u32x4 hi, lo;
             g16_split8(v, hi, lo);
@@ -580,6 +592,7 @@ struct CeOut {
   CeRows rows;
   const unsigned short* tail;              // dx: P's last G16_PAD rows of k where K ends in front of them, or NULL
   int R, C, K, tiles_r, tiles_c, split;
+  int gp;                                  // G's planes: bf16 with two takes them one after the other
   float* part; int64_t slot;               // fp32 [split][C][R], accumulated into where acc is set
   int acc;
   void* out; int out16; int64_t ldo;       // else the final tensor, typed, times 1 / (scale * G's scale)
@@ -652,10 +665,18 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
   const int kb = min(sp * per, nk), ke = min(kb + per, nk);
   G16Acc<NP, CFG> acc;
   g16_tile<NP, CFG, true, QCOL>(acc, p.P, p.Q, tr * C::T, tc * C::T, kb * BK, ke * BK, lds);
+  if (NP == 1 && p.gp == 2) {
+    const G16Op lo = {p.Q.p + p.Q.plane, p.Q.ld, 0, p.Q.rows, p.Q.cols};
+    g16_tile<NP, CFG, true, QCOL, true>(acc, p.P, lo, tr * C::T, tc * C::T, kb * BK, ke * BK, lds);
+  }
   if constexpr (!QCOL) {
     if (p.tail && sp + 1 == p.split) {
       const G16Op tp = {p.tail, p.P.ld, 0, G16_PAD, p.P.cols}, tq = {p.Q.p + p.K, p.Q.ld, p.Q.plane, p.Q.rows, p.Q.cols};
       g16_tile<NP, CFG, true, false, true>(acc, tp, tq, tr * C::T, tc * C::T, 0, G16_PAD, lds);
+      if (NP == 1 && p.gp == 2) {
+        const G16Op lo = {tq.p + tq.plane, tq.ld, 0, tq.rows, tq.cols};
+        g16_tile<NP, CFG, true, false, true>(acc, tp, lo, tr * C::T, tc * C::T, 0, G16_PAD, lds);
+      }
     }
   }
   const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = ce_factor<NP>(p.g);
@@ -690,10 +711,10 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
 // Few rows, bf16: both gradients in one pass over W, without the matrix cores.  A thread has eight columns of x and of dx in registers and
 // walks over the vocabulary: reads its 16 bytes of a row of W, adds G times it to dx, writes G times x to dW.  rp rows of W to a
 // workgroup a time, `per` threads to a row (a power of two; blockIdx.y: columns beyond 4096); every row group leaves a partial dx.
-// Bound by memory: one row against 65536 x 2048 reads and writes 268 MB, 94 us (a copy
+// Bound by memory: one row against 65536 x 2048 reads and writes 268 MB, 97 us (a copy
 // takes 98); the two products take 71 + 88.
 template <int TT>
-__global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __restrict__ w, const unsigned short* __restrict__ G, int64_t ldg,
+__global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __restrict__ w, const unsigned short* __restrict__ G, int64_t ldg, int64_t plane,
                                                      const unsigned short* __restrict__ x, int64_t D, int T, int nv, int per, int acc,
                                                      float* __restrict__ part, int64_t slot, unsigned short* __restrict__ dw, CeGrad g) {
   const int r = threadIdx.x / per, rp = 512 / per;
@@ -719,7 +740,7 @@ __global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __res
       const int64_t v = v0 + u * step < nv ? v0 + u * step : v0;
       q[u] = *reinterpret_cast<const g16_u32x4*>(w + v * D + col);
 #pragma unroll
-      for (int t = 0; t < TT; ++t) gv[u][t] = g16_f32(G[t * ldg + v]);
+      for (int t = 0; t < TT; ++t) gv[u][t] = g16_f32(G[t * ldg + v]) + g16_f32(G[plane + t * ldg + v]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -933,7 +954,7 @@ static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) 
   char* p = (char*)base;
   size_t at = 0;
   b.shared = (float*)p; at += 256;
-  b.G = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * b.piece * 2);
+  b.G = (unsigned short*)(p + at); at += ce_up((size_t)d.gp * d.Tp * b.piece * 2);
   b.slot = d.T * d.Dp;
   b.part = b.split > 1 || b.pieces > 1 ? (float*)(p + at) : nullptr;                    // else dx is written by its product
   if ((want_dx || b.few) && b.part) at += ce_up((size_t)b.split * b.slot * 4);
@@ -975,20 +996,20 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
     a.rows = k.rows; a.bias = bias; a.bias16 = bias16; a.scale = k.scale; a.z = k.z;
     a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing; a.v0 = (int)v0;
-    a.g = cg; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
+    a.g = cg; a.gp = d.gp; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
     if (int rc = ce_logits<true>(a, nv, T, bf16, nullptr, st)) return rc;
     const int64_t gpl = d.Tp * b.piece;
     if (b.few && (dx || dw)) {
       const dim3 g((unsigned)b.blocks, (unsigned)ceil_div(D, b.few * 8));
       unsigned short* dwp = dw ? (unsigned short*)dw + v0 * D : nullptr;
-#define CE_FEW_ROWS(TT) hipLaunchKernelGGL(ce_few_kernel<TT>, g, dim3(512), 0, st, (const unsigned short*)w + v0 * D, b.G, b.piece, k.x, D, (int)T, (int)nv, b.few, i > 0, b.part, b.slot, dwp, cg)
+#define CE_FEW_ROWS(TT) hipLaunchKernelGGL(ce_few_kernel<TT>, g, dim3(512), 0, st, (const unsigned short*)w + v0 * D, b.G, b.piece, gpl, k.x, D, (int)T, (int)nv, b.few, i > 0, b.part, b.slot, dwp, cg)
       if (T == 1) CE_FEW_ROWS(1); else if (T == 2) CE_FEW_ROWS(2); else CE_FEW_ROWS(4);
 #undef CE_FEW_ROWS
       OFQ_LAUNCH_CHECK();
     }
     if (dw && !b.few) {
       CeOut o = {};
-      o.rows = k.rows;
+      o.rows = k.rows; o.gp = d.gp;
       o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.R = (int)D; o.C = (int)nv; o.K = (int)d.Tp; o.split = 1;
@@ -1001,7 +1022,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     }
     if (dx && !b.few) {
       CeOut o = {};
-      o.rows = k.rows;
+      o.rows = k.rows; o.gp = d.gp;
       o.P = ce_w_op(d, k, w, v0);
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.C = (int)T; o.K = (int)kdx; o.split = b.split; o.tail = tail ? k.w : nullptr; o.scale = k.scale + 1; o.g = cg;

@@ -131,6 +131,21 @@ def test_few_rows_of_bf16(T, D, V, ignored, reduction):
     check(call(x, w, b, y, 0.1, reduction, grad), reference(x, w, b, y, 0.1, reduction, grad), "bf16", zmax)
 
 
+@pytest.mark.parametrize("T,D,V", [(1, 64, 2), (2, 96, 3), (3, 128, 700), (33, 96, 130), (64, 320, 75)])
+def test_gradients_of_few_rows_are_off_by_their_own_rounding_alone(T, D, V):
+    """bf16, up to 64 rows: G is held to 16 bits.  An element of a gradient is off by half a step of its own (2^-8 relative) and by what G's two
+    roundings (2^-8 of 2^-8), the logits (products of bf16 are exact, their sums and exponentials off by 2^-20) and fp32 sums leave of
+    sum |G| |W|: together below 2^-15 of that."""
+    x, w, b, y = make(T, D, V, "bf16")
+    got = call(x, w, b, y, 0.1, "sum")
+    want = reference(x, w, b, y, 0.1, "sum")
+    z = x.double() @ w.double().t() + b.double()
+    G = torch.softmax(z, 1) - 0.1 / V
+    G[torch.arange(T), y] -= 0.9
+    for a, c, size in ((got[1], want[1], G.abs() @ w.double().abs()), (got[2], want[2], G.abs().t() @ x.double().abs())):
+        assert bool(((a.double().cpu() - c).abs() <= 2.0 ** -8 * c.abs() + 2.0 ** -15 * size).all())
+
+
 def test_few_rows_with_one_gradient_alone():
     from ofq_amd.functional import linear_cross_entropy
     x, w, _, y = make(2, 128, 500, "bf16")
