@@ -16,7 +16,10 @@
 #define CE_AMAX_X 128                    // partial maxima of x and of W
 #define CE_AMAX_W 384
 #define CE_FINE G16_PAD                  // rows up to which G of bf16 tensors has two planes
-#define CE_FEW 4                         // rows up to which the gradients of bf16 tensors are one pass over W
+// Rows up to which W is read as it is, without the matrix cores.  Few / not, us, both directions, V 65536, D 2048: bf16 1 row 191 / 225, 4 rows
+// 246 / 310, 8 rows 464 / 313; fp32 (whose W would be packed) 1 row 362 / 850, 4 rows 387, 8 rows 542 / 857.
+#define CE_FEW_16 4
+#define CE_FEW 8
 #define CE_PIECE_BYTES (128ll << 20)     // of G: half of the 256 MB last-level cache
 
 static int ce_form(int64_t R, int64_t C, int split) {
@@ -27,19 +30,20 @@ static int ce_form(int64_t R, int64_t C, int split) {
 struct CeDims {
   int64_t T, D, V, Tp, Dp, Vp, tiles_v, tiles_t;
   int np, gp;                // planes of the operands, of G
-  bool pack_w;
+  bool pack_w, few;
 };
 static bool ce_dims(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, CeDims* d) {
   if (T <= 0 || D <= 0 || V <= 0 || T > (1 << 24) || D > (1 << 20) || V > (1 << 24)) return false;
   auto pad = [](int64_t v) { return (v + G16_PAD - 1) / G16_PAD * G16_PAD; };
   d->T = T; d->D = D; d->V = V; d->Tp = pad(T); d->Dp = pad(D); d->Vp = pad(V);
-  d->tiles_v = ceil_div(V, g16_t(ce_form(V, T, 1)));                 // of the forward pass
+  d->few = T <= (bf16 ? CE_FEW_16 : CE_FEW);
+  d->tiles_v = ceil_div(V, d->few ? 64 : g16_t(ce_form(V, T, 1)));   // of the forward pass
   d->tiles_t = ceil_div(T, 64);                                      // at most
   d->np = bf16 ? 1 : 2;
   // G of few bf16 rows is held to 16 bits: where one row's rounding is not averaged with others' it showed in the whole gradient (two rows of
   // three classes: dx 2.3e-3 off, the rounding of the outputs alone 1.6e-3), and their time is W's way from memory.
   d->gp = bf16 && T > CE_FINE ? 1 : 2;
-  d->pack_w = !bf16 || d->Dp != D || !w_aligned;
+  d->pack_w = !d->few && (!bf16 || d->Dp != D || !w_aligned);
   return true;
 }
 static size_t ce_up(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -66,7 +70,7 @@ static int64_t ce_z(const CeDims& d) {
 }
 
 // What the forward pass leaves for the backward.  Rows whose target is ignore_index take no part in anything: the others are packed in
-// their order, n of them.  W planes: zero padded to Vp rows; where W is used in place and its last rows do not fill G16_PAD, those, zero
+// their order, n of them.  Few rows (d.few): x in fp32, the logits [T][V].  Else W planes: zero padded to Vp rows; where W is used in place and its last rows do not fill G16_PAD, those, zero
 // padded.
 struct CeRows { int* n; int* pos; int* idx; int* y; float* lse; };    // [1]; row -> packed row or -1; packed -> row; target or -1; lse
 __host__ __device__ static inline int64_t ce_w_rows(const CeDims& d) { return d.pack_w ? d.Vp : d.Vp != d.V ? G16_PAD : 0; }
@@ -80,9 +84,9 @@ static CeKept ce_kept(void* base, const CeDims& d, bool backward) {
   k.rows.idx = (int*)(p + at); at += ce_up(d.Tp * 4);
   k.rows.y = (int*)(p + at); at += ce_up(d.Tp * 4);
   k.rows.lse = (float*)(p + at); at += ce_up(d.Tp * 4);
-  k.x = (unsigned short*)(p + at); at += ce_up((size_t)d.np * d.Tp * d.Dp * 2);
-  k.w = (unsigned short*)(p + at); at += ce_up((size_t)d.np * ce_w_rows(d) * d.Dp * 2);
-  const int64_t z = backward ? ce_z(d) : 0;
+  k.x = (unsigned short*)(p + at); at += d.few ? ce_up((size_t)CE_FEW * d.D * 4) : ce_up((size_t)d.np * d.Tp * d.Dp * 2);
+  k.w = (unsigned short*)(p + at); at += d.few ? 0 : ce_up((size_t)d.np * ce_w_rows(d) * d.Dp * 2);
+  const int64_t z = !backward ? 0 : d.few ? d.T * d.V : ce_z(d);
   k.z = z ? (float*)(p + at) : nullptr; at += ce_up((size_t)z * 4);
   k.bytes = at;
   return k;
@@ -708,64 +712,245 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
   }
 }
 
-// Few rows, bf16: both gradients in one pass over W, without the matrix cores.  A thread has eight columns of x and of dx in registers and
-// walks over the vocabulary: reads its 16 bytes of a row of W, adds G times it to dx, writes G times x to dW.  rp rows of W to a
-// workgroup a time, `per` threads to a row (a power of two; blockIdx.y: columns beyond 4096); every row group leaves a partial dx.
-// Bound by memory: one row against 65536 x 2048 reads and writes 268 MB, 97 us (a copy
-// takes 98); the two products take 71 + 88.
-template <int TT>
-__global__ __launch_bounds__(512) void ce_few_kernel(const unsigned short* __restrict__ w, const unsigned short* __restrict__ G, int64_t ldg, int64_t plane,
-                                                     const unsigned short* __restrict__ x, int64_t D, int T, int nv, int per, int acc,
-                                                     float* __restrict__ part, int64_t slot, unsigned short* __restrict__ dw, CeGrad g) {
-  const int r = threadIdx.x / per, rp = 512 / per;
-  const int64_t col = ((int64_t)blockIdx.y * per + threadIdx.x % per) * 8;
-  if (col >= D) return;
-  float xs[TT][8], dx[TT][8];
-  float* mine = part + (blockIdx.x * rp + r) * slot + col;
+// ---- few rows: without the matrix cores, W read as it is.  Bound by memory: W once for the logits, once for both gradients.
+template <bool BF16> __device__ __forceinline__ float ce_load(const void* p, int64_t i) {
+  if constexpr (BF16) return g16_f32(reinterpret_cast<const unsigned short*>(p)[i]);
+  else return reinterpret_cast<const float*>(p)[i];
+}
+// N consecutive elements (8 or 16 bytes, aligned), as fp32
+template <bool BF16, int N> __device__ __forceinline__ void ce_load_n(const void* p, int64_t i, float (&v)[N]) {
+  if constexpr (BF16) {
+    unsigned q[N / 2];
+    const unsigned short* a = reinterpret_cast<const unsigned short*>(p) + i;
+    if constexpr (N == 8) *reinterpret_cast<g16_u32x4*>(q) = *reinterpret_cast<const g16_u32x4*>(a);
+    else *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(a);
 #pragma unroll
-  for (int t = 0; t < TT; ++t)
+    for (int e = 0; e < N; ++e) v[e] = __uint_as_float(e & 1 ? q[e >> 1] & 0xffff0000u : q[e >> 1] << 16);
+  } else {
+    const float* a = reinterpret_cast<const float*>(p) + i;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      xs[t][e] = g16_f32(x[t * D + col + e]);
-      dx[t][e] = acc && t < T ? mine[t * D + e] : 0.f;
-    }
-  const float f = ce_factor<1>(g);
-  constexpr int U = 4;
-  const int step = gridDim.x * rp;
-  for (int v0 = blockIdx.x * rp + r; v0 < nv; v0 += U * step) {
-    g16_u32x4 q[U];
-    float gv[U][TT];
+    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(v + e) = *reinterpret_cast<const float4*>(a + e);
+  }
+}
+
+struct CeFew {
+  const void* x; const void* w; const void* bias;
+  CeRows k;
+  float* xs; float* z;                               // kept: the rows that count in fp32 [CE_FEW][D]; logits [T][V], or NULL
+  int64_t D;
+  int bias16, Tp, T, V;
+  float2* part; float* zsum; float* zy;
+  CeGrad g;                                          // backward
+  float* dxp; int64_t slot; void* dw; void* db;
+  int per;
+};
+
+// Logits and their statistics, 64 classes to a workgroup, a wave to four classes a time, its lanes along D.  VEC: 16 bytes a load (every row of
+// W and x is a multiple of that), else an element.  65536 x 2048 bf16, one row: 65 us, 4.1 TB/s.
+template <bool BF16, bool VEC, int TT>
+__global__ __launch_bounds__(256) void ce_few_logits_kernel(CeFew p) {
+  constexpr int N = VEC ? (BF16 ? 8 : 4) : 1, U = TT > 2 ? 4 : 8;
+  __shared__ float zs[TT][64];
+  const int n = *p.k.n, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  if (blockIdx.x == 0)
+    for (int t = 0; t < TT; ++t)
+      for (int64_t i = threadIdx.x; i < p.D; i += 256) p.xs[t * p.D + i] = t < n ? ce_load<BF16>(p.x, (int64_t)p.k.idx[t] * p.D + i) : 0.f;
+  int64_t row[TT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t v = v0 + u * step < nv ? v0 + u * step : v0;
-      q[u] = *reinterpret_cast<const g16_u32x4*>(w + v * D + col);
+  for (int t = 0; t < TT; ++t) row[t] = t < n ? (int64_t)p.k.idx[t] * p.D : -1;
+  const int v0 = blockIdx.x * 64 + wid * 16;
+  for (int g = 0; g < 16; g += U) {
+    float acc[U][TT];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) gv[u][t] = g16_f32(G[t * ldg + v]) + g16_f32(G[plane + t * ldg + v]);
-    }
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v0 + u * step >= nv) break;
-      float o[8];
+      for (int t = 0; t < TT; ++t) acc[u][t] = 0.f;
+    int64_t at[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float we = __uint_as_float(e & 1 ? q[u][e >> 1] & 0xffff0000u : q[u][e >> 1] << 16);
-        float s = 0.f;
+    for (int u = 0; u < U; ++u) at[u] = (int64_t)min(v0 + g + u, p.V - 1) * p.D;
+#pragma unroll 2
+    for (int64_t d = lane * N; d < p.D; d += 64 * N) {
+      float w[U][N];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          dx[t][e] = fmaf(gv[u][t], we, dx[t][e]);
-          s = fmaf(gv[u][t], xs[t][e], s);
-        }
-        o[e] = ce_times(s, f);
+      for (int u = 0; u < U; ++u) {
+        if constexpr (VEC) ce_load_n<BF16, N>(p.w, at[u] + d, w[u]);
+        else w[u][0] = ce_load<BF16>(p.w, at[u] + d);
       }
-      if (dw) *reinterpret_cast<g16_u32x4*>(dw + (v0 + u * step) * D + col) = g16_bf16x8_of(o);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        if (row[t] < 0) continue;
+        float x[N];
+        if constexpr (VEC) ce_load_n<BF16, N>(p.x, row[t] + d, x);
+        else x[0] = ce_load<BF16>(p.x, row[t] + d);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[u][t] = fmaf(w[u][e], x[e], acc[u][t]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        float a = acc[u][t];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
+        if (lane == 0) zs[t][wid * 16 + g + u] = a;
+      }
+  }
+  __syncthreads();
+  const int v = blockIdx.x * 64 + lane;
+  float b = 0.f;
+  if (p.bias && v < p.V) b = p.bias16 ? ce_load<true>(p.bias, v) : ce_load<false>(p.bias, v);
+  for (int t = wid; t < n; t += 4) {
+    const float z = v < p.V ? zs[t][lane] + b : -INFINITY;
+    if (v < p.V && p.z) p.z[(int64_t)t * p.V + v] = z;
+    if (v < p.V && v == p.k.y[t]) p.zy[t] = z;
+    float m = z, sum = v < p.V ? z : 0.f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float e = __expf(z - (m == -INFINITY ? 0.f : m));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { e += __shfl_xor(e, o, 64); sum += __shfl_xor(sum, o, 64); }
+    if (lane == 0) {
+      const int64_t at = (int64_t)blockIdx.x * p.Tp + t;
+      p.part[at] = make_float2(m, e);
+      if (p.zsum) p.zsum[at] = sum;
     }
   }
+}
+
+// All gradients in one pass over W.  A thread has eight columns (four, with more than four rows) of x and of dx in registers and walks over the
+// vocabulary: reads its columns of a row of W, adds G times them to dx, writes G times x to dW.  512 / per rows of W to a workgroup a time,
+// `per` threads to a row (a power of two; blockIdx.y: further columns); every row group leaves a partial dx.  VEC: a thread's columns are
+// consecutive (D is a multiple of 8); else they are `per` apart.  The loads have no conditions (columns past the end read column 0), or each would be waited for.
+// One row against 65536 x 2048 bf16 reads and writes 268 MB in 86 us (a copy takes 98; two products on the matrix cores take 71 + 88).
+template <int TT> constexpr int ce_few_columns() { return TT > 4 ? 4 : 8; }
+template <bool BF16, bool VEC, int TT>
+__global__ __launch_bounds__(512) void ce_few_kernel(CeFew p) {
+  constexpr int N = ce_few_columns<TT>(), U = 4;
+  const int r = threadIdx.x / p.per, rp = 512 / p.per, l = threadIdx.x % p.per, n = *p.k.n, D = (int)p.D;
+  const int first = blockIdx.y * p.per * N;
+  int col[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) col[e] = VEC ? first + l * N + e : first + e * p.per + l;
+  float xs[TT][N], dx[TT][N], w[TT], lse[TT];
+  int y[TT];
+  const float unit = 1.f / ce_unit(p.g.eps), ev = p.g.eps / (float)p.V * unit, on = (1.f - p.g.eps) * unit, f = ce_factor<1>(p.g);
+  const bool finite = fabsf(f) <= 3e38f;             // (else the products are scaled one by one, zeros left alone)
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    y[t] = t < n ? p.k.y[t] : -1;
+    const bool live = t < n && y[t] >= 0;
+    w[t] = !live ? 0.f : p.g.reduction ? 1.f : p.g.grad[p.k.idx[t]] / p.g.shared[0];
+    lse[t] = live ? p.k.lse[t] : 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      xs[t][e] = col[e] < D ? p.xs[t * p.D + col[e]] * (finite ? f : 1.f) : 0.f;
+      dx[t][e] = 0.f;
+    }
+  }
+  const int step = gridDim.x * rp;
+  for (int v0 = blockIdx.x * rp + r; v0 < p.V; v0 += U * step) {
+    float q[U][N], z[U][TT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * step < p.V ? v0 + u * step : v0;
+      const int64_t at = v * p.D;
+      if constexpr (VEC) {
+        ce_load_n<BF16, N>(p.w, at + (col[0] < D ? col[0] : 0), q[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[u][e] = ce_load<BF16>(p.w, at + (col[e] < D ? col[e] : 0));
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) z[u][t] = p.z[(int64_t)(t < n ? t : 0) * p.V + v];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * step;
+      if (v >= p.V) break;
+      const int64_t at = v * p.D;
+      float o[N], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        float gt = (__expf(z[u][t] - lse[t]) * unit - (v == y[t] ? on : 0.f) - ev) * w[t];
+        gt = w[t] == 0.f ? 0.f : gt;
+        sum += gt;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          dx[t][e] = fmaf(gt, q[u][e], dx[t][e]);
+          o[e] = fmaf(gt, xs[t][e], o[e]);
+        }
+      }
+      if (p.dw) {
+        if (!finite) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] = ce_times(o[e], f);
+        }
+        if constexpr (VEC) {
+          if (col[0] < D) {                          // (D is a multiple of 8)
+            if constexpr (BF16 && N == 8) {
+              *reinterpret_cast<g16_u32x4*>(reinterpret_cast<unsigned short*>(p.dw) + at + col[0]) = g16_bf16x8_of(o);
+            } else if constexpr (BF16) {
+              const float o8[8] = {o[0], o[1], o[2], o[3], 0.f, 0.f, 0.f, 0.f};
+              const g16_u32x4 h = g16_bf16x8_of(o8);
+              *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(p.dw) + at + col[0]) = make_uint2(h[0], h[1]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < N; e += 4)
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.dw) + at + col[e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            if (col[e] >= D) continue;
+            if constexpr (BF16) reinterpret_cast<unsigned short*>(p.dw)[at + col[e]] = g16_bf16(o[e]);
+            else reinterpret_cast<float*>(p.dw)[at + col[e]] = o[e];
+          }
+        }
+      }
+      if (p.db && blockIdx.y == 0 && l == 0) {
+        const float s = ce_times(sum, f);
+        if (p.bias16) reinterpret_cast<unsigned short*>(p.db)[v] = g16_bf16(s);
+        else reinterpret_cast<float*>(p.db)[v] = s;
+      }
+    }
+  }
+  if (!p.dxp) return;
 #pragma unroll
   for (int t = 0; t < TT; ++t)
-    if (t < T) {
-      *reinterpret_cast<float4*>(mine + t * D) = make_float4(dx[t][0], dx[t][1], dx[t][2], dx[t][3]);
-      *reinterpret_cast<float4*>(mine + t * D + 4) = make_float4(dx[t][4], dx[t][5], dx[t][6], dx[t][7]);
+    if (t < n) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (col[e] < D) p.dxp[(int64_t)(blockIdx.x * rp + r) * p.slot + t * p.D + col[e]] = dx[t][e];
     }
+}
+
+// dx of few rows: 32 groups of threads share the many partials of eight columns and meet in LDS
+__global__ __launch_bounds__(256) void ce_dx_few_kernel(const float* __restrict__ part, int64_t slot, int split, int64_t T, int64_t D, CeRows k, CeGrad g,
+                                                        void* __restrict__ dx, int out16) {
+  __shared__ float sums[32][8];
+  const int64_t i = blockIdx.x * 8ll + threadIdx.x % 8, t = i / D, c = i - t * D;
+  const int l = threadIdx.x % 8, q = threadIdx.x / 8;
+  const int at = t < T ? k.pos[t] : -1, ns = at < 0 ? 0 : split;
+  float v = 0.f;
+  const float* p = part + at * D + c;
+#pragma unroll 8
+  for (int s = q; s < ns; s += 32) v += p[s * slot];
+  sums[q][l] = v;
+  for (int half = 16; half > 0; half >>= 1) {
+    __syncthreads();
+    if (q < half) sums[q][l] = v += sums[q + half][l];
+  }
+  if (q == 0 && t < T) {
+    v = ce_times(v, ce_factor<1>(g));
+    if (out16) reinterpret_cast<unsigned short*>(dx)[i] = g16_bf16(v);
+    else reinterpret_cast<float*>(dx)[i] = v;
+  }
 }
 
 // dx = sum of the split's partials, in order, scaled and typed, and zeros in the rows that do not count
@@ -789,38 +974,6 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e] * a, b);
     ce_put(dx, out16, t * d.D + c, (int)min((int64_t)8, d.D - c), v);
-  }
-}
-
-// The same where there are few columns and many partials: 32 groups of threads share those of a chunk and meet in LDS
-__global__ __launch_bounds__(256) void ce_dx_few_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, CeRows k, CeGrad g,
-                                                        unsigned short* __restrict__ dx) {
-  __shared__ float sums[32][8][9];
-  const int64_t per = d.Dp / 8, i = blockIdx.x * 8ll + threadIdx.x % 8, t = i / per, c = (i - t * per) * 8;
-  const int l = threadIdx.x % 8, q = threadIdx.x / 8;
-  const int at = t < d.T ? k.pos[t] : -1;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const float* p = part + at * d.Dp + c;
-  const int ns = at < 0 ? 0 : split;
-#pragma unroll 8
-  for (int s = q; s < ns; s += 32) {
-    const float4 x = *reinterpret_cast<const float4*>(p + s * slot), y = *reinterpret_cast<const float4*>(p + s * slot + 4);
-    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sums[q][l][e] = v[e];
-  for (int half = 16; half > 0; half >>= 1) {
-    __syncthreads();
-    if (q < half) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[q][l][e] = v[e] += sums[q + half][l][e];
-    }
-  }
-  if (q == 0 && t < d.T) {
-    const float f = ce_factor<1>(g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e], f);
-    ce_put(dx, 1, t * d.D + c, 8, v);
   }
 }
 
@@ -888,6 +1041,24 @@ static int ce_grad(CeOut& o, int bf16, hipStream_t st) {
   return 0;
 }
 
+template <bool BF16, bool VEC>
+static void ce_few_launch(const CeFew& a, bool backward, dim3 g, hipStream_t st) {
+#define CE_FEW_ROWS(TT)                                                                                              \
+  do {                                                                                                               \
+    if (backward) hipLaunchKernelGGL((ce_few_kernel<BF16, VEC, TT>), g, dim3(512), 0, st, a);                         \
+    else hipLaunchKernelGGL((ce_few_logits_kernel<BF16, VEC, TT>), g, dim3(256), 0, st, a);                           \
+  } while (0)
+  if (a.T == 1) CE_FEW_ROWS(1); else if (a.T == 2) CE_FEW_ROWS(2); else if (BF16 || a.T <= CE_FEW_16) CE_FEW_ROWS(4); else if constexpr (!BF16) CE_FEW_ROWS(8);
+#undef CE_FEW_ROWS
+}
+static int ce_few(const CeFew& a, int bf16, const void* other, bool backward, dim3 g, hipStream_t st) {
+  const bool vec = a.D % (bf16 || backward ? 8 : 4) == 0 && (((uintptr_t)a.w | (uintptr_t)other) & 15) == 0;
+  if (bf16) { if (vec) ce_few_launch<true, true>(a, backward, g, st); else ce_few_launch<true, false>(a, backward, g, st); }
+  else { if (vec) ce_few_launch<false, true>(a, backward, g, st); else ce_few_launch<false, false>(a, backward, g, st); }
+  OFQ_LAUNCH_CHECK();
+  return 0;
+}
+
 // reduction: 0 none (loss [T]), 1 mean, 2 sum (loss: one float)
 extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
                                  int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, int backward, float* loss,
@@ -902,24 +1073,33 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   if (ceil_div(V, 64) * d.tiles_t >= (1ll << 31)) return OFQ_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   float* rows_out = reduction == 0 ? loss : nullptr;
-  if (bf16) hipLaunchKernelGGL(ce_number_kernel, dim3(1), dim3(1024), 0, st, target, ignore_index, T, (int)V, k.rows, rows_out);
+  if (bf16 || d.few) hipLaunchKernelGGL(ce_number_kernel, dim3(1), dim3(1024), 0, st, target, ignore_index, T, (int)V, k.rows, rows_out);
   else hipLaunchKernelGGL(ce_amax_kernel, dim3(CE_AMAX_X + CE_AMAX_W + 1), dim3(256), 0, st, (const float*)x, target, ignore_index, T, D,
                           (int)V, (const float*)w, V * D, f.amax, k.rows, rows_out);
   OFQ_LAUNCH_CHECK();
-  const int64_t chunks = (d.Tp + ce_w_rows(d)) * (d.Dp / 8);
-  const dim3 pg((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 4096));
-  if (bf16) hipLaunchKernelGGL(ce_pack_kernel<1>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
-  else hipLaunchKernelGGL(ce_pack_kernel<2>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
-  OFQ_LAUNCH_CHECK();
-  CeLogits a = {};
-  a.w = ce_w_op(d, k, w, 0);
-  a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
-  a.rows = k.rows; a.bias = bias; a.bias16 = bias16; a.scale = k.scale; a.z = k.z;
-  a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing;
-  a.part = f.part; a.zsum = smoothing != 0.f ? f.zsum : nullptr; a.zy = f.zy;
+  float* zsum = smoothing != 0.f ? f.zsum : nullptr;
   int tv;
-  if (int rc = ce_logits<false>(a, V, T, bf16, &tv, st)) return rc;
-  const CeJoin j = {f.part, a.zsum, f.zy, k.rows, d.Tp, (int)V, tv, reduction, smoothing, f.rows, loss};
+  if (d.few) {
+    CeFew a = {};
+    a.x = x; a.w = w; a.bias = bias; a.bias16 = bias16; a.k = k.rows; a.xs = (float*)k.x; a.z = k.z;
+    a.D = D; a.Tp = (int)d.Tp; a.T = (int)T; a.V = (int)V; a.part = f.part; a.zsum = zsum; a.zy = f.zy;
+    tv = (int)d.tiles_v;
+    if (int rc = ce_few(a, bf16, x, false, dim3((unsigned)tv), st)) return rc;
+  } else {
+    const int64_t chunks = (d.Tp + ce_w_rows(d)) * (d.Dp / 8);
+    const dim3 pg((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 4096));
+    if (bf16) hipLaunchKernelGGL(ce_pack_kernel<1>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
+    else hipLaunchKernelGGL(ce_pack_kernel<2>, pg, dim3(256), 0, st, x, w, d, f.amax, k);
+    OFQ_LAUNCH_CHECK();
+    CeLogits a = {};
+    a.w = ce_w_op(d, k, w, 0);
+    a.x = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
+    a.rows = k.rows; a.bias = bias; a.bias16 = bias16; a.scale = k.scale; a.z = k.z;
+    a.Tp = (int)d.Tp; a.V = (int)V; a.Dp = (int)d.Dp; a.eps = smoothing;
+    a.part = f.part; a.zsum = zsum; a.zy = f.zy;
+    if (int rc = ce_logits<false>(a, V, T, bf16, &tv, st)) return rc;
+  }
+  const CeJoin j = {f.part, zsum, f.zy, k.rows, d.Tp, (int)V, tv, reduction, smoothing, f.rows, loss};
   // little to join: one workgroup does that and the sum, one launch less
   if (T * tv <= 8192) {
     if (tv <= 64) hipLaunchKernelGGL((ce_join_kernel<1024, 128, true>), dim3(1), dim3(1024), 0, st, j);
@@ -933,31 +1113,33 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   return 0;
 }
 
-struct CeBwd { int64_t piece, pieces; int split, few, blocks; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
+struct CeBwd { int64_t piece, pieces; int split, per, columns, blocks; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
 static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) {
-  CeBwd b;
+  CeBwd b = {};
+  if (d.few) {                                       // `per` threads to a row of W, at least four rows to each
+    b.columns = d.T > 4 ? ce_few_columns<CE_FEW>() : ce_few_columns<1>();
+    for (b.per = 8; b.per < 512 && b.per * b.columns < d.D; b.per *= 2) {}
+    b.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(256, ceil_div(d.V, 4 * (512 / b.per))));
+    b.split = b.blocks * (512 / b.per);
+    b.shared = (float*)base;
+    b.part = (float*)((char*)base + 256);
+    b.slot = d.T * d.D;
+    b.bytes = 256 + (want_dx ? ce_up((size_t)b.split * b.slot * 4) : 0);
+    return b;
+  }
   b.pieces = ce_pieces(d, &b.piece);
-  // threads to a row of W where both gradients are one pass over it
-  b.few = b.blocks = 0;
-  if (d.np == 1 && !d.pack_w && d.T <= CE_FEW)
-    for (b.few = 8; b.few < 512 && b.few * 8 < d.D; b.few *= 2) {}
   // dx has few tiles and a long k: split it so that two workgroups to a CU have work, and none waits for a place (24 tiles, k 21888, two
   // planes: 528 workgroups 86 us, 504 61), at no less than eight k-steps each
   const int64_t tiles = ceil_div(d.T, 128) * ceil_div(d.D, 128), steps = b.piece / (d.np == 1 ? 64 : 32);
   // (32 steps of the fp32 head of 1000 classes: 25 us at once, three parts 8 and 5 for the launch that joins them)
   b.split = (int)std::max<int64_t>(1, std::min(512 / tiles, steps / 8));
-  if (b.few) {
-    const int rp = 512 / b.few;
-    b.blocks = (int)std::min<int64_t>(256, ceil_div(b.piece, 4 * rp));
-    b.split = b.blocks * rp;
-  }
   char* p = (char*)base;
   size_t at = 0;
   b.shared = (float*)p; at += 256;
   b.G = (unsigned short*)(p + at); at += ce_up((size_t)d.gp * d.Tp * b.piece * 2);
   b.slot = d.T * d.Dp;
   b.part = b.split > 1 || b.pieces > 1 ? (float*)(p + at) : nullptr;                    // else dx is written by its product
-  if ((want_dx || b.few) && b.part) at += ce_up((size_t)b.split * b.slot * 4);
+  if (want_dx && b.part) at += ce_up((size_t)b.split * b.slot * 4);
   b.db = (float*)(p + at); if (want_db) at += ce_up((size_t)d.tiles_t * b.piece * 4);
   b.bytes = at;
   return b;
@@ -987,6 +1169,17 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     OFQ_LAUNCH_CHECK();
   }
   const CeGrad cg = {grad, k.rows.n, b.shared, reduction, smoothing};
+  if (d.few) {
+    CeFew a = {};
+    a.w = w; a.bias16 = bias16; a.k = k.rows; a.xs = (float*)k.x; a.z = k.z; a.D = D; a.T = (int)T; a.V = (int)V; a.g = cg;
+    a.dxp = dx ? b.part : nullptr; a.slot = b.slot; a.dw = dw; a.db = db; a.per = b.per;
+    if (int rc = ce_few(a, bf16, dw, true, dim3((unsigned)b.blocks, (unsigned)ceil_div(D, b.per * b.columns)), st)) return rc;
+    if (dx) {
+      hipLaunchKernelGGL(ce_dx_few_kernel, dim3((unsigned)ceil_div(T * D, 8)), dim3(256), 0, st, b.part, b.slot, b.split, T, D, k.rows, cg, dx, bf16);
+      OFQ_LAUNCH_CHECK();
+    }
+    return 0;
+  }
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, V - v0);
     const bool tail = !d.pack_w && nv % G16_PAD;                          // (of the last piece: the others are whole tiles)
@@ -999,15 +1192,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     a.g = cg; a.gp = d.gp; a.G = b.G; a.ldg = b.piece; a.db = db ? b.db : nullptr;
     if (int rc = ce_logits<true>(a, nv, T, bf16, nullptr, st)) return rc;
     const int64_t gpl = d.Tp * b.piece;
-    if (b.few && (dx || dw)) {
-      const dim3 g((unsigned)b.blocks, (unsigned)ceil_div(D, b.few * 8));
-      unsigned short* dwp = dw ? (unsigned short*)dw + v0 * D : nullptr;
-#define CE_FEW_ROWS(TT) hipLaunchKernelGGL(ce_few_kernel<TT>, g, dim3(512), 0, st, (const unsigned short*)w + v0 * D, b.G, b.piece, gpl, k.x, D, (int)T, (int)nv, b.few, i > 0, b.part, b.slot, dwp, cg)
-      if (T == 1) CE_FEW_ROWS(1); else if (T == 2) CE_FEW_ROWS(2); else CE_FEW_ROWS(4);
-#undef CE_FEW_ROWS
-      OFQ_LAUNCH_CHECK();
-    }
-    if (dw && !b.few) {
+    if (dw) {
       CeOut o = {};
       o.rows = k.rows; o.gp = d.gp;
       o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
@@ -1020,7 +1205,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
       }
       if (int rc = ce_grad<true>(o, bf16, st)) return rc;
     }
-    if (dx && !b.few) {
+    if (dx) {
       CeOut o = {};
       o.rows = k.rows; o.gp = d.gp;
       o.P = ce_w_op(d, k, w, v0);
@@ -1030,7 +1215,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
       else { o.R = (int)D; o.out = dx; o.out16 = bf16; o.ldo = D; }
       if (int rc = ce_grad<false>(o, bf16, st)) return rc;
     }
-    if (db && (!dw || b.few)) {
+    if (db && !dw) {
       const dim3 g((unsigned)ceil_div(nv, 256));
       const int tl = g16_t(ce_form(nv, T, 1));
       char* to = (char*)db + v0 * (bias16 ? 2 : 4);
@@ -1042,8 +1227,7 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
   if (dx && b.part) {
     const int64_t chunks = T * (d.Dp / 8);
     const dim3 g((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 8192));
-    if (b.few) hipLaunchKernelGGL(ce_dx_few_kernel, dim3((unsigned)ceil_div(chunks, 8)), dim3(256), 0, st, b.part, b.slot, b.split, d, k.rows, cg, (unsigned short*)dx);
-    else if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
+    if (bf16) hipLaunchKernelGGL(ce_dx_kernel<1>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
     else hipLaunchKernelGGL(ce_dx_kernel<2>, g, dim3(256), 0, st, b.part, b.slot, b.split, d, k.scale + 1, k.rows, cg, dx, bf16);
     OFQ_LAUNCH_CHECK();
   }

@@ -117,18 +117,20 @@ def test_many_pieces_of_the_vocabulary(dtype):
     check(got, want, dtype, 16.0)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("ignored", [False, True])
-@pytest.mark.parametrize("T,D,V", [(1, 64, 2), (1, 4160, 300), (2, 128, 5000), (3, 512, 777), (4, 2048, 1030), (4, 8192, 65), (5, 512, 777)])
+@pytest.mark.parametrize("T,D,V", [(1, 64, 2), (1, 4160, 300), (2, 128, 5000), (3, 511, 777), (4, 2048, 1030), (4, 8192, 65), (5, 516, 777), (7, 33, 64),
+                                   (8, 1000, 129), (8, 4100, 500), (9, 512, 777)])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
-def test_few_rows_of_bf16(T, D, V, ignored, reduction):
-    """Up to four rows take both gradients in one pass over the weights: columns beyond 4096, vocabularies smaller than the grid, rows
-    that do not count."""
-    x, w, b, y = make(T, D, V, "bf16")
+def test_few_rows(T, D, V, ignored, reduction, dtype):
+    """Up to eight rows (bf16: four) take the logits and the gradients in one pass over the weights each: rows of whole 16 bytes and others, columns beyond
+    4096, vocabularies smaller than the grid, rows that do not count."""
+    x, w, b, y = make(T, D, V, dtype)
     if ignored and T > 1:
         y[T // 2] = -100
     grad = torch.linspace(-1.0, 2.0, T) if reduction == "none" else None
     zmax = float((x.double() @ w.double().t()).abs().max()) + 2
-    check(call(x, w, b, y, 0.1, reduction, grad), reference(x, w, b, y, 0.1, reduction, grad), "bf16", zmax)
+    check(call(x, w, b, y, 0.1, reduction, grad), reference(x, w, b, y, 0.1, reduction, grad), dtype, zmax)
 
 
 @pytest.mark.parametrize("T,D,V", [(1, 64, 2), (2, 96, 3), (3, 128, 700), (33, 96, 130), (64, 320, 75)])
