@@ -422,7 +422,7 @@ __device__ __forceinline__ void g16_tri(int t, int n, int& r, int& c) {
 }
 
 // The tile form for a grid of so many tiles of 64, 128 and 256.  In units of a 128 tile's time on a CU that has two of them, a 256 tile takes
-// 3.4; every CU takes whole tiles.  Measured (MID / BIG, us): 1024 tiles of 128, k 14336: 495 / 412; 3072, two planes, k 2048: 639 / 590;
+// 3.4; every CU takes whole tiles.  Measured (MID / BIG, us): 1024 tiles of 128, k 14336: 495 / 412; 96 x 32, two planes, k 2048: 639 / 590;
 // 1026, i.e. 260 of 256, two planes: 81 / 93; 512: 125 / 173.  TINY / MID, two planes: 10 tiles of 64, k 192: 6 / 10; 180, k 192 and 768:
 // 12 / 19; 474, k 197: 11 / 14; 540, k 192: 16 / 14; 2160: 63 / 45.  DEEP / MID: 180 of 128, k 384: 23 / 25.
 static inline int g16_form(int64_t t64, int64_t t128, int64_t t256) {
