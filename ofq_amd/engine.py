@@ -327,11 +327,6 @@ class GraphedTrainStep:
     The first `warmup` calls run eagerly (real training steps: lazily created state -- optimizer moments, workspaces,
     CGA masks -- must exist before the capture); the next call captures and replays."""
 
-    # what a capture next to a live process group does (see _capture); tools/capture_stress.py flips these to reproduce the
-    # watchdog crash of round 4
-    capture_error_mode_dp = "thread_local"
-    drain_before_capture = True
-
     def __init__(self, model, optimizer, loss_fn=None, dp=None, cga=None, warmup=2, alias_inputs=False, mode="full"):
         if not hasattr(optimizer, "advance_for_replay"):
             raise RuntimeError("GraphedTrainStep needs ofq_amd.optim.FusedAdamW (per-step scalars in device memory)")
@@ -389,12 +384,11 @@ class GraphedTrainStep:
             # With a process group alive, c10d's watchdog thread polls the end events of the collectives it has not retired yet
             # (hipEventQuery every 100 ms).  Under capture mode "global" every thread's event queries count as capture errors
             # while ANY thread captures, and on this stack that ends the process ("operation not permitted on an event last
-            # recorded in a capturing stream", raised in the watchdog: tools/capture_stress.py reproduces it).  So: only this
+            # recorded in a capturing stream", raised in the watchdog).  So: only this
             # thread's calls count (thread_local), and the capture starts only after every collective issued so far reports
             # completion through its own Work handle (bounded, raises on timeout -- no blind sleep).
-            mode = self.capture_error_mode_dp
-            if self.drain_before_capture:
-                self.dp.drain_collectives()
+            mode = "thread_local"
+            self.dp.drain_collectives()
         if self.mode == "segmented":
             self._capture_segmented(images, target, soft_target, mode)
             g = self.segments[0][0]
