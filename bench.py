@@ -70,9 +70,9 @@ def parse():
     ap.add_argument("--no-graph", action="store_true",
                     help="launch every kernel from Python each step instead of replaying the captured hipGraph of the step")
     ap.add_argument("--graph", action="store_true",
-                    help="with several ranks: capture the RCCL collectives inside the step's graph as well (default there: "
-                         "captured compute in sub-graphs cut at the gradient buckets, each bucket's all-reduce issued eagerly "
-                         "behind its sub-graph; the capture of collectives is validated with one rank only, tests/test_graph_gpu.py)")
+                    help="with several ranks: the captured step (the default there as well: captured compute in sub-graphs cut at the "
+                         "gradient buckets, each bucket's all-reduce issued eagerly behind its sub-graph; collectives are never "
+                         "captured, engine.GraphedTrainStep)")
     ap.add_argument("--split-graph", action="store_true",
                     help="with several ranks: round 4's form -- one graph for the whole backward, then every bucket all-reduce "
                          "(exposed), then the optimiser graph -- instead of the sub-graphs cut at the bucket boundaries")
@@ -351,20 +351,18 @@ def main():
         return engine.train_step(model, opt, images, target, soft_targets(), loss_fn, dp=dp, cga=cga)
 
     eager_step = step
-    # one rank: graph replay of the whole step.  Several ranks: graph replay of the compute with the bucket all-reduces issued
-    # eagerly between two graphs (RCCL collectives inside a hipGraph could only be exercised with one rank on the one-GPU
-    # development boxes: --graph), so that the host issues a handful of launches per step instead of ~850 next to RCCL's proxy
-    # threads; --no-graph is the eager path (collectives overlapped with backward, 20 ms of Python per step).
+    # one rank: graph replay of the whole step.  Several ranks (or --force-dp): graph replay of the compute in sub-graphs cut at
+    # the bucket boundaries, each bucket's all-reduce issued eagerly behind its sub-graph and overlapped with the next one, so
+    # that the host issues a handful of launches per step instead of ~850 next to RCCL's proxy threads (--split-graph: all
+    # collectives after the whole backward graph; --no-graph: the eager path, collectives overlapped with backward, 20 ms of
+    # Python per step).
     use_graph = not args.no_graph
-    # with the data-parallel wrapper (several ranks, or --force-dp): "split" = captured compute + eager collectives
-    # (engine.GraphedTrainStep) unless --graph asks for the collectives inside the graph
-    # ("segmented": graph A cut at the bucket boundaries, each bucket's all-reduce issued behind its sub-graph and overlapped
-    # with the next one; --split-graph keeps round 4's form: all collectives after the whole backward graph)
-    graph_mode = "full" if (dp is None or args.graph) else ("split" if args.split_graph else "segmented")
+    graph_mode = "split" if args.split_graph and not args.graph else "segmented"      # ("full" where there is nothing to reduce)
     n_warm = args.warmup
     if use_graph:
         # same step, device side replayed from a hipGraph: the first two calls run eagerly, the third captures
         gstep = engine.GraphedTrainStep(model, opt, loss_fn, dp=dp, cga=cga, warmup=2, alias_inputs=True, mode=graph_mode)
+        graph_mode = gstep.mode
         n_warm = max(args.warmup, gstep.warmup + 1)          # the capture must not fall into the timed region
 
         def step():

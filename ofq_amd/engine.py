@@ -310,11 +310,20 @@ def _latch_quantizers(model):
     return [(m, q) for m in model.modules() for q in [getattr(m, "input_quant_fn", None)] if isinstance(q, LsqQuantizer4img)]
 
 
+def _capture_error_mode():
+    """With a process group alive c10d's watchdog thread queries events (hipEventQuery every 100 ms) at any time; under mode "global" that
+    is a capture error and ends the process.  Only the capturing thread's own calls may count then, whether or not the step that is captured
+    has a DataParallel of its own."""
+    import torch.distributed as dist
+    return "thread_local" if dist.is_available() and dist.is_initialized() else "global"
+
+
 class GraphedTrainStep:
     """train_step() with the device side of the step captured once in a hipGraph and replayed: one hipGraphLaunch instead of
     ~850 ctypes launches and ~20 ms of Python per step (the C ABI is capture-safe by construction: no allocation, no sync,
     no global state; torch's allocator serves the capture from a private pool, so every activation, gradient and workspace
-    address is the same in every replay).
+    address is the same in every replay).  With a synchronised DataParallel (dp.sync) the collectives run eagerly between
+    sub-graphs: mode "full" is carried out as "segmented" then.
 
     What is NOT in the graph, because it changes from step to step on the host:
       * lr and the AdamW bias corrections -- FusedAdamW keeps them in device memory and advance_for_replay() rewrites
@@ -333,20 +342,24 @@ class GraphedTrainStep:
         if mode not in ("full", "split", "segmented"):
             raise ValueError("mode must be 'full', 'split' or 'segmented'")
         self.model, self.optimizer, self.dp, self.cga = model, optimizer, dp, cga
-        # mode "split" (the default of bench.py / train.py with several ranks): captured compute, eager collectives --
-        #   graph A = zero_grad + StatsQ refresh + forward + loss + backward + the packing of the gradient buckets,
-        #   then the bucket all-reduces issued eagerly on RCCL's stream (DataParallel.all_reduce_packed),
-        #   graph B = [CGA masks] + AdamW [+ CGA restore].
-        # No collective is ever captured (RCCL inside a hipGraph has only been exercised with one rank here), the host issues
-        # two graph launches and one collective per bucket per step instead of ~850 kernel launches, and the all-reduce is
-        # exposed (90.8 MB of gradients over xGMI: well under a millisecond of a 22 ms step) instead of overlapped.
-        # mode "segmented" (the default of bench.py / train.py with several ranks since round 5): graph A is cut at the bucket
-        # boundaries -- the capture is ended and a new one begun inside the gradient hook that packs a bucket -- and bucket i's
-        # all-reduce is issued eagerly right after sub-graph i has been launched: RCCL's stream waits for exactly that
-        # sub-graph and reduces next to sub-graph i+1 (train.py:727's "all-reduce overlapped with backward" at ~2 host calls
-        # per bucket); only the last bucket's collective is exposed.  The backward pass of the capture runs on the calling
-        # thread (torch.autograd.set_multithreading_enabled(False)): a capture is ended by the thread that began it.
-        self.mode = mode if (dp is not None and dp.sync) else "full"
+        # With a synchronised DataParallel no collective is ever captured.  A captured collective puts RCCL's own stream into the capture,
+        # while c10d's watchdog thread still polls (every 100 ms) the end events of eager collectives recorded on that stream: an event
+        # last recorded in a capturing stream may not be queried, the watchdog throws, and the process ends.  Work.is_completed() says that a
+        # collective is done, not that the watchdog has let go of its event, and c10d has nothing to wait for that; so the
+        # collectives stay outside, whatever else has been issued on RCCL's stream and by whom.
+        # mode "segmented" (the default with several ranks; "full" becomes it): graph A = zero_grad + StatsQ refresh + forward + loss +
+        #   backward + the packing of the gradient buckets, cut at the bucket boundaries -- the capture is ended and a new one begun inside the
+        #   gradient hook that packs a bucket; bucket i's all-reduce is issued eagerly right after sub-graph i has been launched: RCCL's stream
+        #   waits for exactly that sub-graph and reduces next to sub-graph i+1 (train.py:727's "all-reduce overlapped with backward"
+        #   at ~2 host calls per bucket); only the last bucket's collective is exposed; then graph B = [CGA masks] + AdamW [+ CGA
+        #   restore].  The backward pass of the capture runs on the calling thread (torch.autograd.set_multithreading_enabled(False)): a
+        #   capture is ended by the thread that began it.
+        # mode "split": graph A in one piece, then the bucket all-reduces (DataParallel.all_reduce_packed), then graph B; the all-reduce
+        #   (90.8 MB of gradients over xGMI: well under a millisecond of a 22 ms step) is exposed instead of overlapped.
+        if dp is None or not dp.sync:
+            self.mode = "full"
+        else:
+            self.mode = "segmented" if mode == "full" else mode
         self.segments = []                       # [(graph, [bucket indices packed inside it])]
         self.verify_replays = 3                  # replays after which the ranks compare their reduced gradients (world > 1)
         self.graph_b = None
@@ -379,15 +392,10 @@ class GraphedTrainStep:
         self.optimizer.zero_grad(set_to_none=True)
         g = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
-        mode = "global"
+        mode = _capture_error_mode()
         if self.dp is not None and self.dp.sync:
-            # With a process group alive, c10d's watchdog thread polls the end events of the collectives it has not retired yet
-            # (hipEventQuery every 100 ms).  Under capture mode "global" every thread's event queries count as capture errors
-            # while ANY thread captures, and on this stack that ends the process ("operation not permitted on an event last
-            # recorded in a capturing stream", raised in the watchdog).  So: only this
-            # thread's calls count (thread_local), and the capture starts only after every collective issued so far reports
-            # completion through its own Work handle (bounded, raises on timeout -- no blind sleep).
-            mode = "thread_local"
+            # the capture starts only after every collective issued so far reports completion through its own Work handle
+            # (bounded, raises on timeout -- no blind sleep)
             self.dp.drain_collectives()
         if self.mode == "segmented":
             self._capture_segmented(images, target, soft_target, mode)

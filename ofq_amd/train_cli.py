@@ -65,8 +65,8 @@ def build_parser(cga=False):
                    help='all-reduce the StatsQ scale vectors behind the last gradient bucket of every step and assert that it '
                         'is a no-op (they are functions of replica-identical weights; the reference has no such collective)')
     p.add_argument('--graph', action='store_true',
-                   help='capture the step in a hipGraph also when several ranks train together (the captured RCCL all-reduce '
-                        'has only been exercised with one rank: without this flag multi-rank runs launch eagerly, like bench.py)')
+                   help='replay the captured step (the default; with several ranks the collectives run between its sub-graphs and are '
+                        'never captured)')
     # quantisation flags (train.py:297-366)
     p.add_argument('--quantized', action='store_true')
     p.add_argument('--wq-enable', action='store_true')
@@ -280,12 +280,10 @@ def main_worker(local_rank, args, cga, spawned):
     hooks = engine.CGAHooks(model, args.wq_bitw, args.boundaryRange, qk_reparam=qkr, model_type=args.model_type) if cga else None
     first, last = (args.epochs, args.epochs + args.freeze_for_n_epochs) if cga else (start_epoch, args.epochs + args.cooldown_epochs)
     graphed = None
-    multi_rank = dp is not None and getattr(dp, "world", 1) > 1
     if not args.no_graph and hasattr(optimizer, "advance_for_replay"):
         # several ranks: captured compute in sub-graphs cut at the gradient buckets, each bucket's all-reduce issued eagerly behind
-        # its sub-graph and overlapped with the next (--graph: collectives captured too)
-        graphed = engine.GraphedTrainStep(model, optimizer, loss_fn, dp=dp, cga=hooks,
-                                          mode="segmented" if (multi_rank and not args.graph) else "full")
+        # its sub-graph and overlapped with the next
+        graphed = engine.GraphedTrainStep(model, optimizer, loss_fn, dp=dp, cga=hooks, mode="segmented")
     no_soft = torch.zeros(args.batch_size, args.num_classes, device=dev)
     for epoch in range(first, last):                                                        # cga.py:760 / train.py:816
         model.train()
