@@ -561,11 +561,13 @@ int ofq_input_pipeline_u8(const uint8_t* in, float* out, int64_t B, int64_t C, i
  *  kept: what the backward needs beside its arguments (ofq_linear_ce_kept_bytes; w_aligned = w is a multiple of 16 bytes; backward = 0:
  *  none is to come; the backward pass refuses another size than its own), ws: scratch; both 256-byte aligned device memory of the caller.
  *  bwd: grad = the incoming gradient (one float; reduction 0: [T]); dx [T][D], dw [V][D] in the tensors' type, db [V] in the
- *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.
+ *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.  reduction 0: the rows' gradients may
+ *  be of any size next to each other (a row of dx is right to its own).
  *  T <= 2^24, V <= 2^24, D <= 2^20. */
 size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, int backward);
 size_t ofq_linear_ce_fwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16);
-size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int want_dx, int want_db);
+size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int want_dx, int want_db);      /* enough for any reduction */
+size_t ofq_linear_ce_bwd_call_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int reduction, int want_dx, int want_dw, int want_db);
 int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias, const int64_t* target, int64_t T, int64_t D, int64_t V,
                       int bf16, int bias16, int64_t ignore_index, float smoothing, int reduction, int backward, float* loss,
                       void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, ofq_stream_t stream);

@@ -136,6 +136,7 @@ SIGNATURES = {
     "ofq_linear_ce_kept_bytes": (sz, [i64, i64, i64, i32, i32, i32]),
     "ofq_linear_ce_fwd_ws_bytes": (sz, [i64, i64, i64, i32]),
     "ofq_linear_ce_bwd_ws_bytes": (sz, [i64, i64, i64, i32, i32, i32]),
+    "ofq_linear_ce_bwd_call_ws_bytes": (sz, [i64, i64, i64, i32, i32, i32, i32, i32]),
     "ofq_linear_ce_fwd": (i32, [vp, vp, vp, vp, i64, i64, i64, i32, i32, i64, f32, i32, i32, vp, vp, sz, vp, sz, vp]),
     "ofq_linear_ce_bwd": (i32, [vp, vp, vp, vp, sz, i64, i64, i64, i32, i32, f32, i32, vp, vp, vp, vp, sz, vp]),
     "ofq_newton_schulz_entry_bytes": (i64, []),

@@ -72,7 +72,8 @@ static int64_t ce_z(const CeDims& d) {
 // What the forward pass leaves for the backward.  Rows whose target is ignore_index take no part in anything: the others are packed in
 // their order, n of them.  Few rows (d.few): x in fp32, the logits [T][V].  Else W planes: zero padded to Vp rows; where W is used in place and its last rows do not fill G16_PAD, those, zero
 // padded.
-struct CeRows { int* n; int* pos; int* idx; int* y; float* lse; };    // [1]; row -> packed row or -1; packed -> row; target or -1; lse
+// [1]; row -> packed row or -1; packed -> row; target or -1; lse; fp32 in planes: a row's largest element (by row, those that count)
+struct CeRows { int* n; int* pos; int* idx; int* y; float* lse; float* xmax; };
 __host__ __device__ static inline int64_t ce_w_rows(const CeDims& d) { return d.pack_w ? d.Vp : d.Vp != d.V ? G16_PAD : 0; }
 struct CeKept { float* scale; CeRows rows; unsigned short* x; unsigned short* w; float* z; size_t bytes; };
 static CeKept ce_kept(void* base, const CeDims& d, bool backward) {
@@ -84,6 +85,7 @@ static CeKept ce_kept(void* base, const CeDims& d, bool backward) {
   k.rows.idx = (int*)(p + at); at += ce_up(d.Tp * 4);
   k.rows.y = (int*)(p + at); at += ce_up(d.Tp * 4);
   k.rows.lse = (float*)(p + at); at += ce_up(d.Tp * 4);
+  k.rows.xmax = (float*)(p + at); at += d.np == 2 && !d.few ? ce_up(d.Tp * 4) : 0;
   k.x = (unsigned short*)(p + at); at += d.few ? ce_up((size_t)CE_FEW * d.D * 4) : ce_up((size_t)d.np * d.Tp * d.Dp * 2);
   k.w = (unsigned short*)(p + at); at += d.few ? 0 : ce_up((size_t)d.np * ce_w_rows(d) * d.Dp * 2);
   const int64_t z = !backward ? 0 : d.few ? d.T * d.V : ce_z(d);
@@ -177,7 +179,11 @@ __global__ __launch_bounds__(256) void ce_amax_kernel(const float* __restrict__ 
   if (blockIdx.x < CE_AMAX_X) {
     for (int64_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < T; t += CE_AMAX_X * 4) {
       if (y[t] == ignore) continue;
-      for (int64_t i = threadIdx.x & 63; i < D; i += 64) m = fmaxf(m, fabsf(x[t * D + i]));
+      float r = 0.f;
+      for (int64_t i = threadIdx.x & 63; i < D; i += 64) r = fmaxf(r, fabsf(x[t * D + i]));
+      r = ofq_wave_max(r);
+      if ((threadIdx.x & 63) == 0) k.xmax[t] = r;
+      m = fmaxf(m, r);
     }
   } else {
     const int64_t n4 = ((uintptr_t)w & 15) == 0 ? nw / 4 : 0;
@@ -252,11 +258,17 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ x
   }
 }
 
-// The incoming gradient as the backward launches see it.  reduction mean / sum: one float for all rows; none: one a row, their largest in
-// shared[0].  G holds (exp(z - lse) - (1 - e)[v = y] - e/V) / unit, times a row's share of the largest gradient: what all rows have in
-// common is multiplied in fp32 at the end.  A target's element, the one that carries a gradient, is then -1 for a class that is not
-// learnt yet, which 16 bits hold exactly; 1/n or 1 - e rounded to bf16 would be one relative error, up to 2^-9, common to all rows, that
-// no sum averages (dW and dx of 4096 rows in bf16: 2.8e-3 from the formula in 64 bits, against 1.8e-3 so).
+// The incoming gradient as the backward launches see it.  reduction mean / sum: one float for all rows; none: one a row.
+// What all rows have in common is multiplied in fp32 at the end: G holds (exp(z - lse) - (1 - e)[v = y] - e/V) / unit.  A target's element,
+// the one that carries a gradient, is then -1 for a class that is not learnt yet, which 16 bits hold exactly; 1/n or 1 - e rounded to bf16
+// would be one relative error, up to 2^-9, common to all rows, that no sum averages (dW and dx of 4096 rows in bf16: 2.8e-3 from
+// the formula in 64 bits, against 1.8e-3 so).
+// A row's own gradient: bf16 G, whose exponents are fp32's, takes it along, over the largest (shared[0]).  fp32's two fp16 planes hold an
+// element down to 2^-17 of the largest in full and none below 2^-38: rows' gradients of unlike size would cost the small rows of dx
+// their digits (1e-6 of the largest: 2e-4 of that row's dx).  There G is without it; dx, a row at a time, is multiplied by it in
+// fp32 at the end, and dW, db are sums over rows of it times x, times 1: x is packed once more with it (ce_weighted_kernel), scaled by what
+// the largest of the products needs.  shared: [0] a power of two next to the largest gradient, [1] the packed products' scale, [2] that
+// over x's own.
 struct CeGrad {
   const float* grad; const int* n; const float* shared;
   int reduction;
@@ -265,10 +277,16 @@ struct CeGrad {
 __device__ __forceinline__ float ce_unit(float eps) { return eps <= 0.5f ? 1.f - eps : 1.f; }
 // two planes: |G| <= 2^14, as the scaled operands are
 template <int NP> __device__ __forceinline__ constexpr float ce_gscale() { return NP == 2 ? 8192.f : 1.f; }
-template <int NP> __device__ __forceinline__ float ce_factor(const CeGrad& g) {
+// what the sums are multiplied by at the end (behind the planes' scales, which come off first: a power of two more next to a small factor would
+// take its last places)
+__device__ __forceinline__ float ce_factor(const CeGrad& g) {
   const float n = (float)*g.n;
   const float common = g.reduction == 0 ? g.shared[0] : g.reduction == 2 ? g.grad[0] : n > 0.f ? g.grad[0] / n : 0.f;
-  return common * ce_unit(g.eps) * (1.f / ce_gscale<NP>());
+  return common * ce_unit(g.eps);
+}
+// of row t of dx
+template <int NP> __device__ __forceinline__ float ce_factor_row(const CeGrad& g, int64_t t) {
+  return NP == 2 && g.reduction == 0 ? g.grad[t] * ce_unit(g.eps) : ce_factor(g);
 }
 // a sum of nothing stays zero under an infinite gradient: rows that are ignored, classes behind a mask
 __device__ __forceinline__ float ce_times(float v, float f) { return v == 0.f ? 0.f : v * f; }
@@ -425,13 +443,17 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
       if (p.zsum) p.zsum[at] = stat[2][0][tid] + stat[2][1][tid];
     }
   } else {
-    const float unit = 1.f / ce_unit(p.eps), gs = p.g.reduction ? ce_gscale<NP>() : ce_gscale<NP>() / p.g.shared[0];
+    const bool weighted = NP == 2 && p.g.reduction == 0;
+    const float unit = 1.f / ce_unit(p.eps), gs = NP == 2 || p.g.reduction ? ce_gscale<NP>() : 1.f / p.g.shared[0];
+    float* srow = stat[0][0];                             // the rows' own gradients, for the column sums (a barrier lies in the store below)
+    if (DB && weighted && tid < TL) srow[tid] = c0 + tid < n && p.rows.y[c0 + tid] >= 0 ? p.g.grad[p.rows.idx[c0 + tid]] * (1.f / p.g.shared[0]) : 0.f;
     const float ev = p.eps / (float)p.V * unit, on = (1.f - p.eps) * unit;
 #pragma unroll
     for (int j = 0; j < C::CB; ++j) {
       const int c = c0 + g16_c<CFG>(wc, j, lane);
       const bool live = c < n && p.rows.y[c] >= 0;
-      const float w = !live ? 0.f : p.g.reduction ? gs : p.g.grad[p.rows.idx[c]] * gs, lse = live ? p.rows.lse[c] : 0.f;
+      const float own = live && !p.g.reduction ? p.g.grad[p.rows.idx[c]] : 1.f, lse = live ? p.rows.lse[c] : 0.f;
+      const float w = !live || own == 0.f ? 0.f : NP == 2 || p.g.reduction ? gs : own * gs;
       const float wu = w * unit, we = -ev * w, wy = -on * w;
 #pragma unroll
       for (int i = 0; i < C::RB; ++i)
@@ -456,8 +478,9 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
         [&](int c, int r, const float (&v)[8]) {
           const int64_t row = c0 + c, col = tr * TL + r;
           if constexpr (DB) {
+            const float own = weighted ? srow[c] : 1.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) colsum[e] += v[e];
+            for (int e = 0; e < 8; ++e) colsum[e] += v[e] * own;
           }
           if (row >= p.Tp || col >= p.ldg) return;
           unsigned short* dst = p.G + row * p.ldg + col;
@@ -576,7 +599,7 @@ __global__ __launch_bounds__(NT) void ce_join_kernel(CeJoin p) {
 }
 __global__ __launch_bounds__(1024) void ce_reduce_kernel(CeJoin p) { ce_reduce<1024>(p); }
 
-// The largest of rows' own gradients (1 where that is 0, Inf, NaN or has no reciprocal): one workgroup
+// The largest of rows' own gradients (1 where that is 0, Inf or NaN, or it or its reciprocal no normal number): one workgroup
 __global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict__ grad, CeRows k, float* __restrict__ shared) {
   __shared__ float red[16];
   float m = 0.f;
@@ -587,7 +610,53 @@ __global__ __launch_bounds__(1024) void ce_weight_kernel(const float* __restrict
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-    shared[0] = m >= 1e-37f && m <= 1e37f ? m : 1.f;
+    shared[0] = m >= 0x1p-126f && m <= 0x1p126f ? m : 1.f;
+  }
+}
+
+// The same for rows in planes: two passes over the rows, the second for the largest product of a row's gradient and its largest element
+__global__ __launch_bounds__(1024) void ce_weight_rows_kernel(const float* __restrict__ grad, CeRows k, const float* __restrict__ scale, float* __restrict__ shared) {
+  __shared__ float red[16];
+  const int n = *k.n;
+  auto largest = [&](auto&& of) {
+    float m = 0.f;
+    for (int t = threadIdx.x; t < n; t += 1024)
+      if (k.y[t] >= 0) m = fmaxf(m, of(k.idx[t]));
+    m = ofq_wave_max(m);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, red[i]);
+    return m;
+  };
+  const float m = largest([&](int t) { return fabsf(grad[t]); });
+  const int ex = (int)((__float_as_uint(m) >> 23) & 0xffu);
+  const float w = !(m > 0.f) || ex == 255 ? 1.f : __uint_as_float((unsigned)min(max(ex, 1), 253) << 23);      // (its reciprocal is a float too)
+  const float s = scale[0], xw = largest([&](int t) { return fabsf(grad[t]) * (1.f / w) * (k.xmax[t] * s); });
+  const float f = fminf(ce_scale(xw), 0x1p126f / s);
+  if (threadIdx.x == 0) { shared[0] = w; shared[1] = s * f; shared[2] = f; }
+}
+
+// x's planes times the rows' own gradients, for dW; rows without one (or with a target outside the vocabulary) are zeros, whatever x holds.
+// Bound by memory: 8 bytes an element each way.
+__global__ __launch_bounds__(256) void ce_weighted_kernel(const float* __restrict__ grad, const unsigned short* __restrict__ x, CeDims d, CeRows k,
+                                                          const float* __restrict__ shared, unsigned short* __restrict__ out) {
+  const int rows = *k.n;
+  const int64_t per = d.Dp / 8, n = ce_padded(rows) * per, plane = d.Tp * d.Dp;
+  const float inv = 1.f / shared[0], f = shared[2];
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t row = i / per;
+    const float w = row < rows && k.y[row] >= 0 ? grad[k.idx[row]] * inv : 0.f;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (w != 0.f) {
+      g16_join8(*reinterpret_cast<const g16_u32x4*>(x + i * 8), *reinterpret_cast<const g16_u32x4*>(x + plane + i * 8), v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * w * f;
+    }
+    g16_u32x4 hi, lo;
+    g16_split8(v, hi, lo);
+    *reinterpret_cast<g16_u32x4*>(out + i * 8) = hi;
+    *reinterpret_cast<g16_u32x4*>(out + plane + i * 8) = lo;
   }
 }
 
@@ -631,7 +700,7 @@ __device__ __forceinline__ void ce_put_db(const float* __restrict__ cols, int64_
   const int ny = (ce_padded(*g.n) + TL - 1) / TL;
 #pragma unroll 8
   for (int k = 0; k < ny; ++k) s += cols[k * ldg + c];
-  s = ce_times(s, ce_factor<NP>(g));
+  s = ce_times(s * (1.f / ce_gscale<NP>()), ce_factor(g));
   if (out16) reinterpret_cast<unsigned short*>(db)[c] = g16_bf16(s);
   else reinterpret_cast<float*>(db)[c] = s;
 }
@@ -683,7 +752,7 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
       }
     }
   }
-  const float a = NP == 2 ? 1.f / p.scale[0] : 1.f, b = ce_factor<NP>(p.g);
+  const float a = NP == 2 ? 1.f / p.scale[0] * (1.f / ce_gscale<NP>()) : 1.f, b = ce_factor(p.g);
   g16_store_tile<NP, CFG, false>([&](int i, int j, int e) { return acc[i][j][e]; },
                  [&](int c, int r, const float (&v0)[8]) {
                    const int64_t row = tc * C::T + c;
@@ -700,9 +769,11 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_grad_kernel(CeOut p) {
                      }
                      ce_put(o, 0, 0, 8, v);
                    } else {
+                     const int64_t to = QCOL ? row : (int64_t)p.rows.idx[row];
+                     const float f = QCOL || NP == 1 ? b : ce_factor_row<NP>(p.g, to);
 #pragma unroll
-                     for (int e = 0; e < 8; ++e) v[e] = ce_times(v0[e] * a, b);
-                     ce_put(p.out, p.out16, (QCOL ? row : (int64_t)p.rows.idx[row]) * p.ldo + col, p.R - col, v);
+                     for (int e = 0; e < 8; ++e) v[e] = ce_times(v0[e] * a, f);
+                     ce_put(p.out, p.out16, to * p.ldo + col, p.R - col, v);
                    }
                  },
                  [](int, int, const float (&)[8]) {}, lds);
@@ -836,7 +907,7 @@ __global__ __launch_bounds__(512) void ce_few_kernel(CeFew p) {
   for (int e = 0; e < N; ++e) col[e] = VEC ? first + l * N + e : first + e * p.per + l;
   float xs[TT][N], dx[TT][N], w[TT], lse[TT];
   int y[TT];
-  const float unit = 1.f / ce_unit(p.g.eps), ev = p.g.eps / (float)p.V * unit, on = (1.f - p.g.eps) * unit, f = ce_factor<1>(p.g);
+  const float unit = 1.f / ce_unit(p.g.eps), ev = p.g.eps / (float)p.V * unit, on = (1.f - p.g.eps) * unit, f = ce_factor(p.g);
   const bool finite = fabsf(f) <= 3e38f;             // (else the products are scaled one by one, zeros left alone)
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
@@ -947,7 +1018,7 @@ __global__ __launch_bounds__(256) void ce_dx_few_kernel(const float* __restrict_
     if (q < half) sums[q][l] = v += sums[q + half][l];
   }
   if (q == 0 && t < T) {
-    v = ce_times(v, ce_factor<1>(g));
+    v = ce_times(v, ce_factor(g));
     if (out16) reinterpret_cast<unsigned short*>(dx)[i] = g16_bf16(v);
     else reinterpret_cast<float*>(dx)[i] = v;
   }
@@ -958,7 +1029,7 @@ template <int NP>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int64_t slot, int split, CeDims d, const float* __restrict__ scale,
                                                     CeRows k, CeGrad g, void* __restrict__ dx, int out16) {
   const int64_t per = d.Dp / 8, n = d.T * per;
-  const float a = NP == 2 ? 1.f / scale[0] : 1.f, b = ce_factor<NP>(g);
+  const float a = NP == 2 ? 1.f / scale[0] * (1.f / ce_gscale<NP>()) : 1.f;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t t = i / per, c = (i - t * per) * 8;
     if (c >= d.D) continue;
@@ -971,6 +1042,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
       const float4 x = *reinterpret_cast<const float4*>(p + s * slot), y = *reinterpret_cast<const float4*>(p + s * slot + 4);
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
+    const float b = ce_factor_row<NP>(g, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = ce_times(v[e] * a, b);
     ce_put(dx, out16, t * d.D + c, (int)min((int64_t)8, d.D - c), v);
@@ -1113,8 +1185,13 @@ extern "C" int ofq_linear_ce_fwd(const void* x, const void* w, const void* bias,
   return 0;
 }
 
-struct CeBwd { int64_t piece, pieces; int split, per, columns, blocks; float* shared; unsigned short* G; float* part; int64_t slot; float* db; size_t bytes; };
-static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) {
+struct CeBwd {
+  int64_t piece, pieces;
+  int split, per, columns, blocks;
+  float* shared; unsigned short* G; float* part; int64_t slot; float* db; unsigned short* xw; size_t bytes;
+};
+// want_weighted: dW of rows with gradients of their own
+static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db, bool want_weighted) {
   CeBwd b = {};
   if (d.few) {                                       // `per` threads to a row of W, at least four rows to each
     b.columns = d.T > 4 ? ce_few_columns<CE_FEW>() : ce_few_columns<1>();
@@ -1141,6 +1218,7 @@ static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) 
   b.part = b.split > 1 || b.pieces > 1 ? (float*)(p + at) : nullptr;                    // else dx is written by its product
   if (want_dx && b.part) at += ce_up((size_t)b.split * b.slot * 4);
   b.db = (float*)(p + at); if (want_db) at += ce_up((size_t)d.tiles_t * b.piece * 4);
+  b.xw = (unsigned short*)(p + at); if (want_weighted && d.np == 2) at += ce_up((size_t)d.np * d.Tp * d.Dp * 2);
   b.bytes = at;
   return b;
 }
@@ -1148,7 +1226,12 @@ static CeBwd ce_bwd_ws(void* base, const CeDims& d, bool want_dx, bool want_db) 
 extern "C" size_t ofq_linear_ce_bwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int want_dx, int want_db) {
   CeDims d;
   if (!ce_dims(T, D, V, bf16, 1, &d)) return 0;
-  return ce_bwd_ws(nullptr, d, want_dx != 0, want_db != 0).bytes;
+  return ce_bwd_ws(nullptr, d, want_dx != 0, want_db != 0, true).bytes;
+}
+extern "C" size_t ofq_linear_ce_bwd_call_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16, int reduction, int want_dx, int want_dw, int want_db) {
+  CeDims d;
+  if (!ce_dims(T, D, V, bf16, 1, &d)) return 0;
+  return ce_bwd_ws(nullptr, d, want_dx != 0, want_db != 0, reduction == 0 && want_dw != 0).bytes;
 }
 
 // grad: the incoming gradient, one float or (reduction 0) [T]; kept as a forward pass with backward != 0 left it; dx / dw / db: any may be NULL
@@ -1161,10 +1244,19 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     return OFQ_EINVAL;
   const CeKept k = ce_kept((void*)kept, d, true);
   if (kept_bytes != k.bytes) return OFQ_EINVAL;          // another size, or weights that moved to another alignment since
-  const CeBwd b = ce_bwd_ws(ws, d, dx != nullptr, db != nullptr);
+  const bool own = reduction == 0 && !bf16 && !d.few;    // rows' own gradients beside G, not in it
+  const CeBwd b = ce_bwd_ws(ws, d, dx != nullptr, db != nullptr, own && dw != nullptr);
   if (ws_bytes < b.bytes) return OFQ_ENOWS;
   hipStream_t st = (hipStream_t)stream;
-  if (reduction == 0) {
+  if (own) {
+    hipLaunchKernelGGL(ce_weight_rows_kernel, dim3(1), dim3(1024), 0, st, grad, k.rows, k.scale, b.shared);
+    OFQ_LAUNCH_CHECK();
+    if (dw) {
+      const dim3 g((unsigned)std::min<int64_t>(ceil_div(d.Tp * (d.Dp / 8), 256), 4096));
+      hipLaunchKernelGGL(ce_weighted_kernel, g, dim3(256), 0, st, grad, k.x, d, k.rows, b.shared, b.xw);
+      OFQ_LAUNCH_CHECK();
+    }
+  } else if (reduction == 0) {
     hipLaunchKernelGGL(ce_weight_kernel, dim3(1), dim3(1024), 0, st, grad, k.rows, b.shared);
     OFQ_LAUNCH_CHECK();
   }
@@ -1195,10 +1287,10 @@ extern "C" int ofq_linear_ce_bwd(const float* grad, const void* w, const void* b
     if (dw) {
       CeOut o = {};
       o.rows = k.rows; o.gp = d.gp;
-      o.P = G16Op{k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
+      o.P = G16Op{own ? b.xw : k.x, d.Dp, d.Tp * d.Dp, (int)d.Tp, (int)d.Dp};
       o.Q = G16Op{b.G, b.piece, gpl, (int)d.Tp, (int)b.piece};
       o.R = (int)D; o.C = (int)nv; o.K = (int)d.Tp; o.split = 1;
-      o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = k.scale; o.g = cg;
+      o.out = (char*)dw + v0 * D * (bf16 ? 2 : 4); o.out16 = bf16; o.ldo = D; o.scale = own ? b.shared + 1 : k.scale; o.g = cg;
       if (db) {
         o.cols = b.db; o.cols_tl = g16_t(ce_form(nv, T, 1));
         o.db = (char*)db + v0 * (bias16 ? 2 : 4); o.db16 = bias16;

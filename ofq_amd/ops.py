@@ -1467,7 +1467,7 @@ def linear_ce_bwd(grad, weight, bias, kept, T, smoothing, reduction, want_dx=Tru
     dx = torch.empty((T, D), dtype=weight.dtype, device=dev) if want_dx else None
     dw = torch.empty_like(weight) if want_dw else None
     db = torch.empty_like(bias) if want_db and bias is not None else None
-    ws = _scratch(L.ofq_linear_ce_bwd_ws_bytes(T, D, V, b16, int(dx is not None), int(db is not None)), dev)
+    ws = _scratch(L.ofq_linear_ce_bwd_call_ws_bytes(T, D, V, b16, reduction, int(dx is not None), int(dw is not None), int(db is not None)), dev)
     with _Timed("linear cross entropy, backward", 6.0 * T * D * V):
         _chk(L.ofq_linear_ce_bwd(grad.data_ptr(), weight.data_ptr(), _p(bias), kept.data_ptr(), kept.numel(), T, D, V, b16,
                                  int(bias is not None and bias.dtype == torch.bfloat16), smoothing, reduction, _p(dx), _p(dw), _p(db),
