@@ -1313,14 +1313,14 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     piece of the vocabulary at a time."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, smoothing, reduction):
+    def forward(ctx, x, weight, bias, target, ignore_index, smoothing, reduction, backward):
         D = x.shape[-1]
         red = ops.CE_REDUCTIONS[reduction]
         x2d, y = x.reshape(-1, D).contiguous(), target.reshape(-1).contiguous()
         w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
         with ops.on_device(x.device):
-            loss, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red, any(ctx.needs_input_grad[:3]))
+            loss, kept = ops.linear_ce_fwd(x2d, w, b, y, ignore_index, smoothing, red, backward)
         ctx.save_for_backward(w, b, kept)
         ctx.args = (x.shape, y.numel(), smoothing, red)
         return loss.view(target.shape) if red == 0 else loss
@@ -1335,7 +1335,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         with ops.on_device(w.device):
             dx, dw, db = ops.linear_ce_bwd(g.reshape(-1).contiguous(), w, b, kept, T, smoothing, red, want_dx=need[0], want_dw=need[1],
                                            want_db=need[2])
-        return dx.view(shape) if dx is not None else None, dw, db, None, None, None, None
+        return dx.view(shape) if dx is not None else None, dw, db, None, None, None, None, None
 
 
 def linear_cross_entropy(input, weight, target, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
@@ -1369,4 +1369,6 @@ def linear_cross_entropy(input, weight, target, bias=None, ignore_index=-100, la
     if target.numel() == 0:                     # no rows: a sum of nothing (its gradients are zeros), and a mean over nothing
         total = input.float().sum() + weight[:0].float().sum() + (0.0 if bias is None else bias[:0].float().sum())
         return total.expand(target.shape) if reduction == "none" else total if reduction == "sum" else total * float("nan")
-    return LinearCrossEntropyFn.apply(input, weight, bias, target, int(ignore_index), float(label_smoothing), reduction)
+    # (asked here: inside the Function gradients are off, and needs_input_grad is true of a parameter under no_grad too)
+    backward = torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    return LinearCrossEntropyFn.apply(input, weight, bias, target, int(ignore_index), float(label_smoothing), reduction, backward)
