@@ -106,11 +106,11 @@ __device__ __forceinline__ float ce_block_max(float m, float* red) {
 }
 
 // the power of two that brings m into [2^13, 2^14): two planes hold every element down to m 2^-13 with 2^-22 of it, and a
-// rounding up stays far below fp16's 65504; 1 for 0, Inf and NaN
+// rounding up stays far below fp16's 65504; 1 for 0, Inf and NaN.  It and its reciprocal are normal numbers.
 __device__ __forceinline__ float ce_scale(float m) {
   const int ex = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127;
   if (!(m > 0.f) || ex == 128) return 1.f;
-  const int e = min(max(13 - ex, -100), 100);
+  const int e = min(13 - ex, 126);                        // (-114 for the largest m)
   return __uint_as_float((unsigned)(e + 127) << 23);
 }
 
@@ -359,13 +359,14 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
   // What few tiles need (a bias, rows past the vocabulary, a target) is passed over as a whole where it is not there: the epilogue of
   // 256 x 256 logits takes a wave's instructions as long as three k-steps.
   if constexpr (NP == 2) {
-    const float ix = 1.f / p.scale[0], iw = 1.f / p.scale[1];       // powers of two: exact
+    // powers of two, taken off in one step: their product may lie outside fp32's range where the logit does not
+    const int off = 254 - (int)(__float_as_uint(p.scale[0]) >> 23) - (int)(__float_as_uint(p.scale[1]) >> 23);
 #pragma unroll
     for (int i = 0; i < C::RB; ++i)
 #pragma unroll
       for (int j = 0; j < C::CB; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i][j][e] * ix * iw;
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], off);
   }
   if (p.bias) {
 #pragma unroll
