@@ -131,7 +131,10 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ 
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-  const float inv = (float)((double)NS_SCALE / (norm > (double)eps || norm != norm ? norm : (double)eps));
+  // the factor as a power of two and a float in [0.5, 1): as one float it is Inf where norm and eps lie below 3e-36 (and 0 Inf a NaN), and has
+  // no digits left where norm lies above 1e41
+  int ex;
+  const float inv = (float)frexp((double)NS_SCALE / (norm > (double)eps || norm != norm ? norm : (double)eps), &ex);
   const int bc = r.np / NS_BLK, id = blockIdx.x - r.e0;
   const int xr = (id / bc) * NS_BLK, xc = (id % bc) * NS_BLK;          // block of X [mp][np]
   const bool tr = r.rows > r.cols;
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ 
   for (int row = threadIdx.x >> 3; row < NS_BLK; row += 32) {
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (tr ? blk[q + e][row] : blk[row][q + e]) * inv;
+    for (int e = 0; e < 8; ++e) v[e] = ldexpf(tr ? blk[q + e][row] : blk[row][q + e], ex) * inv;
     g16_u32x4 h, l;
     g16_split8(v, h, l);
     const int64_t at = (int64_t)(xr + row) * r.np + xc + q;
