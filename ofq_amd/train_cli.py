@@ -166,11 +166,13 @@ def load_checkpoint(model, path, strict=True, map_location="cpu"):
     return model.load_state_dict(sd, strict=strict)
 
 
-def check_supported(args):
-    """Flags the reference accepts that this path does not implement must not be dropped silently."""
+def check_supported(args, cga=False):
+    """Flags the reference accepts that this path does not implement must not be dropped silently (cga: cga.py's run)."""
     bad = []
     if args.opt.lower() not in ("adamw", "muon"):
         bad.append("--opt %s (adamw: train_scripts/*, configs/*.yml; or muon)" % args.opt)
+    if cga and args.opt.lower() == "muon":
+        bad.append("--opt muon with cga.py (its freeze leaves single elements of the hidden weights out, which an orthogonalised update cannot)")
     if args.sched != "cosine":
         bad.append("--sched %s (only cosine)" % args.sched)
     if (args.mixup > 0 or args.cutmix > 0) and args.mixup_mode != "batch":
@@ -197,7 +199,7 @@ def main_worker(local_rank, args, cga, spawned):
     from . import engine, ops, parallel
     from .deit import create_model
     from .quantization.utils import KDLossSoftandHard, KLLossSoft
-    check_supported(args)
+    check_supported(args, cga)
     if spawned:
         world = int(args.world_size)
         rank = local_rank
