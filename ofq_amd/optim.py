@@ -18,10 +18,11 @@ from . import ops
 
 class _GraphClass:
     """Parameters of one group that have taken the same number of steps: one captured launch, one device scalar block."""
-    __slots__ = ("group", "params", "hyper")
+    __slots__ = ("group", "params", "hyper", "fixed")
 
     def __init__(self, group, params, hyper):
         self.group, self.params, self.hyper = group, params, hyper
+        self.fixed = None            # settings that the captured launches hold by value (FusedMuon)
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -243,7 +244,8 @@ class FusedMuon(FusedAdamW):
     s = sqrt(max(1, rows / columns)) (adjust_lr_fn None or "original") or 0.2 sqrt(max(rows, columns)) ("match_rms_adamw": an update of
     AdamW's size, so that both rules take the same lr).  All matrices of a group go through the same launches.
     A group with use_muon=False is updated by FusedAdamW's rule (betas, adamw_eps): embeddings, heads, vectors.  Parameters are
-    contiguous fp32 on a HIP device; Muon groups hold matrices only.  Captured steps work as FusedAdamW's do."""
+    contiguous fp32 on a HIP device; Muon groups hold matrices only.  Captured steps work as FusedAdamW's do: a Muon group's follow lr and
+    weight_decay, and refuse a replay after a change of its other settings."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NS_COEFFICIENTS, eps=1e-7,
                  ns_steps=5, adjust_lr_fn=None, betas=(0.9, 0.999), adamw_eps=1e-8):
@@ -287,6 +289,21 @@ class FusedMuon(FusedAdamW):
         r, c = shape
         return 0.2 * math.sqrt(max(r, c)) if group["adjust_lr_fn"] == "match_rms_adamw" else math.sqrt(max(1.0, r / c))
 
+    _FIXED = ("momentum", "nesterov", "ns_coefficients", "eps", "ns_steps", "adjust_lr_fn")
+
+    def _capture_muon(self, group):
+        """The device scalars of a captured Muon group's launches; everything else they hold by value."""
+        hyper = self._captured_hyper(group, None)
+        self._graph_classes[-1].fixed = [group[k] for k in self._FIXED]
+        return hyper
+
+    def advance_for_replay(self):
+        for gc in self._graph_classes or ():
+            if gc.fixed is not None and gc.fixed != [gc.group[k] for k in self._FIXED]:
+                raise RuntimeError("FusedMuon: a captured step follows lr and weight_decay; %s changed since: capture the step again"
+                                   % ", ".join(k for k, old in zip(self._FIXED, gc.fixed) if gc.group[k] != old))
+        super().advance_for_replay()
+
     def _advance_class(self, gc):
         if not gc.group["use_muon"]:
             return super()._advance_class(gc)
@@ -323,7 +340,7 @@ class FusedMuon(FusedAdamW):
                 rows = runs[dev] = []
             rows.append((g.data_ptr(), buf.data_ptr(), p.data_ptr(), shape[0], shape[1], scale, 0.0))
         for dev, rows in runs.items():
-            hyper = self._captured_hyper(group, None).data_ptr() if capturing else None
+            hyper = self._capture_muon(group).data_ptr() if capturing else None
             with ops.on_device(dev):
                 ops.newton_schulz(np.array(rows, dtype=ops.NS_ENTRY), False, group["ns_steps"], group["ns_coefficients"], group["eps"],
                                   float(group["lr"]), float(group["weight_decay"]), float(group["momentum"]), group["nesterov"], hyper,
