@@ -20,6 +20,7 @@
 // no load behind a per-element condition (one memory round trip each) -- per-row terms go through LDS, old values
 // for C += ... are fetched unconditionally on clamped addresses.
 #include "common.h"
+#include "qgemm_chunks.h"
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));

@@ -30,8 +30,8 @@ __global__ __launch_bounds__(512) void qgemm_bf16s_nt_wide_kernel(QGemmArgs p) {
   const unsigned short* pb[NB];
   bool okB[NB];
   // a row may be shorter than a k-step (K = 8, 16, 24): the lanes whose chunk lies past it read the row's first chunk, which the
-  // zero k-scale (A) / the zero A operand (B) takes out of the product
-  const int kqa0 = (tid & 7) * 4 < K ? (tid & 7) * 4 : 0, kqb0 = (tid & 3) * 8 < K ? (tid & 3) * 8 : 0;
+  // zero k-scale (A) / the zero mask (B) takes out of the product (qgemm_chunks.h)
+  const int kqa0 = qbs_chunk0((tid & 7) * 4, K), kqb0 = qbs_chunk0((tid & 3) * 8, K);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (tid + 512 * i) >> 3;
@@ -39,14 +39,14 @@ __global__ __launch_bounds__(512) void qgemm_bf16s_nt_wide_kernel(QGemmArgs p) {
 #ifdef NTW_SAME_ROWS
     pa[i] = A + (int64_t)row * p.lda + kqa0;         // experiment: every workgroup reads rows 0..127 (L2 hits)
 #else
-    pa[i] = A + (int64_t)min(m0 + row, p.M - 1) * p.lda + kqa0;
+    pa[i] = A + (int64_t)qbs_row(m0, row, p.M) * p.lda + kqa0;
 #endif
   }
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const int row = (tid + 512 * i) >> 2;
     okB[i] = (n0 + row) < p.N;
-    pb[i] = B + (int64_t)min(n0 + row, p.N - 1) * p.ldb + kqb0;
+    pb[i] = B + (int64_t)qbs_row(n0, row, p.N) * p.ldb + kqb0;
   }
   const int kqa = (tid & 7) * 4, kqb = (tid & 3) * 8;
   float sE = 1.f, inv_sE = 1.f;        // F16: the launch's power of two (see qgemm_bf16s_nt_wide_sk_kernel)
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(512) void qgemm_bf16s_nt_wide_kernel(QGemmArgs p) {
     constexpr int sl = decltype(SLOT)::value;
     const int k0 = kt * QBS_BK;
     rka[sl] = (k0 + kqa) < K;                           // K % 8 == 0 (host check): chunks are all-in or all-out
-    const int ka = rka[sl] ? k0 : 0;
+    const int ka = qbs_step(kqa, k0, K);
     // no scale vector: the load still happens (from the dY panel, any valid address) and the value is replaced at the
     // LDS store; a load under `if (p.s)` ends in a register copy that has to wait for it, i.e. s_waitcnt vmcnt(0) here
     rks[sl] = *reinterpret_cast<const f32x4v*>(p.s ? p.s + ka + kqa0 : pa[0]);
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(512) void qgemm_bf16s_nt_wide_kernel(QGemmArgs p) {
   auto gload_b = [&](int kt) {
     const int k0 = kt * QBS_BK;
     rkb = (k0 + kqb) < K;
-    const int kb = rkb ? k0 : 0;
+    const int kb = qbs_step(kqb, k0, K);
 #pragma unroll
     for (int i = 0; i < NB; ++i) rb[i] = *reinterpret_cast<const i32x4*>(pb[i] + kb);
   };
@@ -248,14 +248,14 @@ __global__ __launch_bounds__(512) void qgemm_bf16s_nt_wide_kernel(QGemmArgs p) {
         *reinterpret_cast<i32x4*>(&nxt[NS * PLANE + row * QBS_LD + kqb * 2]) = rb[i];
       } else if constexpr (P < 2 * NPA + 2 * NB) {
         constexpr int i = P - 2 * NPA - NB;
-        rb[i] = *reinterpret_cast<const i32x4*>(pb[i] + ((kb2 + kqb) < K ? kb2 : 0));
+        rb[i] = *reinterpret_cast<const i32x4*>(pb[i] + qbs_step(kqb, kb2, K));
       } else {
         constexpr int w = P - 2 * NPA - 2 * NB;
         if constexpr (w == 0) {
           rka[sl] = (ka3 + kqa) < K;
-          rks[sl] = *reinterpret_cast<const f32x4v*>(p.s ? p.s + (rka[sl] ? ka3 : 0) + kqa0 : pa[0]);
+          rks[sl] = *reinterpret_cast<const f32x4v*>(p.s ? p.s + qbs_step(kqa, ka3, K) + kqa0 : pa[0]);
         } else {
-          ra[sl][w - 1] = *reinterpret_cast<const f32x4v*>(pa[w - 1] + (rka[sl] ? ka3 : 0));
+          ra[sl][w - 1] = *reinterpret_cast<const f32x4v*>(pa[w - 1] + qbs_step(kqa, ka3, K));
         }
       }
     };

@@ -207,14 +207,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 3
     const int f = tid + 256 * i;
     const int row = f >> 3;
     okA[i] = (m0 + row) < p.M;
-    offA[i] = (int64_t)min(m0 + row, p.M - 1) * p.lda + (f & 7) * 4;
+    offA[i] = (int64_t)qbs_row(m0, row, p.M) * p.lda + (f & 7) * 4;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int f = tid + 256 * i;
     const int row = f >> 2;
     okB[i] = (n0 + row) < p.N;
-    offB[i] = (int64_t)min(n0 + row, p.N - 1) * p.ldb + (f & 3) * 8;
+    offB[i] = (int64_t)qbs_row(n0, row, p.N) * p.ldb + (f & 3) * 8;
   }
   const int kqa = (tid & 7) * 4;       // same for all 4 chunks (256 % 8 == 0)
   const int kqb = (tid & 3) * 8;
@@ -232,16 +232,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 3
   auto gload = [&](int kt) {
     const int k0 = kt * QBS_BK;
     const bool kina = (k0 + kqa) < K, kinb = (k0 + kqb) < K;       // K % 8 == 0 (host check)
-    rks = *reinterpret_cast<const f32x4v*>(ksp ? ksp + (kina ? k0 + kqa : 0) : A + offA[0] - kqa);      // no ksp: any valid address
+    rks = *reinterpret_cast<const f32x4v*>(ksp ? ksp + qbs_chunk(kqa, k0, K) : A + offA[0] - kqa);      // no ksp: any valid address
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ra[i] = *reinterpret_cast<const f32x4v*>(A + offA[i] + (kina ? k0 : -kqa));
+    for (int i = 0; i < 4; ++i) ra[i] = *reinterpret_cast<const f32x4v*>(A + offA[i] + qbs_chunk_from_c(kqa, k0, K));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (!B_I8) {
 #pragma unroll
-        for (int r = 0; r < NB; ++r) rb[r][i] = *reinterpret_cast<const i32x4*>(B + r * p.sBp + offB[i] + (kinb ? k0 : -kqb));
+        for (int r = 0; r < NB; ++r) rb[r][i] = *reinterpret_cast<const i32x4*>(B + r * p.sBp + offB[i] + qbs_chunk_from_c(kqb, k0, K));
       } else {
-        const u32x2v v = *reinterpret_cast<const u32x2v*>(B8 + offB[i] + (kinb ? k0 : -kqb));
+        const u32x2v v = *reinterpret_cast<const u32x2v*>(B8 + offB[i] + qbs_chunk_from_c(kqb, k0, K));
         rb[0][i].x = (int)v[0];
         rb[0][i].y = (int)v[1];
       }
