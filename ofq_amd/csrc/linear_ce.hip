@@ -453,8 +453,8 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ce_logits_kernel(CeLogits p) {
     for (int j = 0; j < C::CB; ++j) {
       const int c = c0 + g16_c<CFG>(wc, j, lane);
       const bool live = c < n && p.rows.y[c] >= 0;
-      const float own = live && !p.g.reduction ? p.g.grad[p.rows.idx[c]] : 1.f, lse = live ? p.rows.lse[c] : 0.f;
-      const float w = !live || own == 0.f ? 0.f : NP == 2 || p.g.reduction ? gs : own * gs;
+      float w = !live ? 0.f : p.g.reduction ? gs : p.g.grad[p.rows.idx[c]] * gs, lse = live ? p.rows.lse[c] : 0.f;
+      if (NP == 2 && !p.g.reduction) w = w == 0.f ? 0.f : gs;
       const float wu = w * unit, we = -ev * w, wy = -on * w;
 #pragma unroll
       for (int i = 0; i < C::RB; ++i)
