@@ -60,8 +60,8 @@ template <int NP, int CFG> struct G16 {
   static constexpr int KS = BK / 16;                    // phases (of 16 k) in a stage
   static constexpr int CPR = BK / 8;                    // 16-byte chunks of a row tile's row
   static constexpr int RPL = 16 / CPR;                  // rows to a 256-byte bank line
-  static constexpr int HALVES = NP * T * BK;            // of one operand's stage: 16 or 32 KB
-  static constexpr int LOADS = HALVES / 1024 / WC;      // DMA loads of a wave and operand for a stage: four
+  static constexpr int HALVES = NP * T * BK;            // of one operand's stage: 8 KB (TINY), 16 or 32 (BIG)
+  static constexpr int LOADS = HALVES / 1024 / WC;      // DMA loads of a wave and operand for a stage: four (TINY: two)
   // the XOR of a col tile's chunks: four k rows on different banks (a row of T = 64 is half a bank line)
   static __device__ constexpr int colx(int k) { return T >= 128 ? (k & 3) << 2 : (k >> 1 & 1) << 2; }
   static constexpr int DEPTH = CFG == G16_DEEP || CFG == G16_TINY ? 4 : 2;       // stages
@@ -163,8 +163,8 @@ __device__ __forceinline__ void g16_read(G16Frags<NP, CFG>& f, const G16Lds& s, 
   else f.b[q][i - RB] = g16_frag<NP, CFG, QCOL>(s.q[buf], q, wc * CB + i - RB, ks, lane);
 }
 // MFMA number n of RB CB (NP = 1) or 3 RB CB (hi hi, hi lo, lo hi).  Inside an MFMA products are cut off some bits below the accumulator's
-// last place (its final rounding is to nearest).  Accumulators of 32 to 128 k each, added up with v_add_f32, halve the error of long
-// sums.  TINY has them: its time is a latency.  In the other forms they took 9 %; there the Newton-Schulz chain is 1.1e-6 to 2.9e-6 off where
+// last place (its final rounding is to nearest).  Accumulators of four stages each (128 k of two planes, 256 of one), added up
+// with v_add_f32, halve the error of long sums.  TINY has them: its time is a latency.  In the other forms they took 9 %; there the Newton-Schulz chain is 1.1e-6 to 2.9e-6 off where
 // fp32 products are 1.5e-6 to 3.9e-6 off, so they are left out.
 template <int NP, int CFG, int N>
 __device__ __forceinline__ void g16_mma(G16Acc<NP, CFG>& acc, const G16Frags<NP, CFG>& f) {
