@@ -48,6 +48,19 @@ __device__ __forceinline__ const NsRec& ns_find(const NsRec* t, int n, int id, F
 }
 
 struct NsStep { float lr, decay, omm; int nesterov; };      // omm = 1 - momentum
+struct NsChain { float a, b, c, eps; int steps; };
+
+// |U|_F of a matrix, from its partial sums; all 256 threads
+__device__ __forceinline__ double ns_norm_of(const NsRec& r, const double* __restrict__ parts) {
+  __shared__ double red[4];
+  double s = (int)threadIdx.x < r.nparts ? parts[r.part + threadIdx.x] : 0.0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return sqrt((red[0] + red[1]) + (red[2] + red[3]));
+}
+__device__ __forceinline__ double ns_divisor(double norm, float eps) { return norm > (double)eps || norm != norm ? norm : (double)eps; }
 
 template <bool BF16>
 __device__ __forceinline__ float ns_load(const void* g, int64_t i) {
@@ -117,24 +130,30 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsRec* __restrict__ 
   if (threadIdx.x == 0) parts[r.part + blockIdx.x - r.p0] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// Of a vector (one row or column) the chain is a scalar's, X = f U: f <- f (a + b A + c A A) with A = (f |U|)^2, here in 64 bits.  In planes and
+// fp32 its error is one factor, common to all of the vector, that nothing averages: 1.1e-6 where plain fp32 products have 0.5e-6.
+__device__ __forceinline__ double ns_vector_factor(double norm, const NsChain& ch) {
+  double f = 1.0 / ns_divisor(norm, ch.eps);
+  for (int k = 0; k < ch.steps; ++k) {
+    const double q = (f * norm) * (f * norm);
+    f *= ch.a + q * (ch.b + q * ch.c);
+  }
+  return f;
+}
+
 // X planes = u / max(|u|_F, eps) * 2^10, transposed where rows > columns, zero padded to [mp][np].  64 x 64 blocks through LDS.  25 million
 // elements in 67 us, 3 TB/s: scalar loads, as either side may be the transposed one.
 template <bool BF16>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const NsRec* __restrict__ t, int n, NsStep st, float eps,
                                                       const double* __restrict__ parts, _Float16* __restrict__ ws) {
   __shared__ float blk[NS_BLK][NS_BLK + 1];
-  __shared__ double red[4];
   const NsRec r = ns_find(t, n, blockIdx.x, [](const NsRec& r) { return r.e0; });
-  double s = (int)threadIdx.x < r.nparts ? parts[r.part + threadIdx.x] : 0.0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+  if (r.m == 1) return;
+  const double norm = ns_norm_of(r, parts);
   // the factor as a power of two and a float in [0.5, 1): as one float it is Inf where norm and eps lie below 3e-36 (and 0 Inf a NaN), and has
   // no digits left where norm lies above 1e41
   int ex;
-  const float inv = (float)frexp((double)NS_SCALE / (norm > (double)eps || norm != norm ? norm : (double)eps), &ex);
+  const float inv = (float)frexp((double)NS_SCALE / ns_divisor(norm, eps), &ex);
   const int bc = r.np / NS_BLK, id = blockIdx.x - r.e0;
   const int xr = (id / bc) * NS_BLK, xc = (id % bc) * NS_BLK;          // block of X [mp][np]
   const bool tr = r.rows > r.cols;
@@ -259,12 +278,37 @@ __global__ __launch_bounds__(g16_nt(CFG)) void ns_update_kernel(const NsRec* __r
 // out = O (the update's own type), or the parameter p <- p decay - lr wscale O; hyper: {lr, decay} from device memory (a captured
 // step), guard: the step's guard word (see adamw.hip).  HBM-bound: 25 million elements in 64 us, 4.6 TB/s.
 template <bool BF16>
-__global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__ t, int n, NsStep st, const float* __restrict__ hyper,
-                                                       const unsigned* __restrict__ guard, int odd, const _Float16* __restrict__ ws) {
+__global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__ t, int n, NsStep st, NsChain ch, const float* __restrict__ hyper,
+                                                       const unsigned* __restrict__ guard, const double* __restrict__ parts,
+                                                       const _Float16* __restrict__ ws) {
   if (guard != nullptr && (__hip_atomic_load(guard, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & 0x7fffffffu) != 0u) return;
   __shared__ float blk[NS_BLK][NS_BLK + 1];
   const NsRec r = ns_find(t, n, blockIdx.x, [](const NsRec& r) { return r.e0; });
   const float lr = hyper ? hyper[0] : st.lr, decay = hyper ? hyper[1] : st.decay;
+  auto put = [&](int64_t at, float o) {
+    if (r.mom) {
+      float* p = reinterpret_cast<float*>(r.out) + at;
+      *p = *p * decay - lr * r.wscale * o;
+    } else if (BF16) {
+      reinterpret_cast<unsigned short*>(r.out)[at] = g16_bf16(o);
+    } else {
+      reinterpret_cast<float*>(r.out)[at] = o;
+    }
+  };
+  if (r.m == 1) {
+    const double f = ns_vector_factor(ns_norm_of(r, parts), ch);
+    const int at = (blockIdx.x - r.e0) * NS_BLK + (int)threadIdx.x;
+    if (threadIdx.x < NS_BLK && at < r.n) {
+      float u = ns_load<BF16>(r.g, at);
+      if (r.mom) {
+        const float m = r.mom[at];
+        u = st.nesterov ? m - st.omm * (m - u) : m;
+      }
+      put(at, (float)(u * f));
+    }
+    return;
+  }
+  const int odd = ch.steps & 1;
   const int bc = r.np / NS_BLK, id = blockIdx.x - r.e0;
   const int xr = (id / bc) * NS_BLK, xc = (id % bc) * NS_BLK;
   const bool tr = r.rows > r.cols;
@@ -284,28 +328,18 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const NsRec* __restrict__
   __syncthreads();
   const int gr = tr ? xc : xr, gc = tr ? xr : xc;
   const int lc = threadIdx.x & 63;
-  const float f = lr * r.wscale;
 #pragma unroll 4
   for (int l = threadIdx.x >> 6; l < NS_BLK; l += 4) {
     const int i = gr + l, j = gc + lc;
     if (i >= r.rows || j >= r.cols) continue;
-    const int64_t at = (int64_t)i * r.cols + j;
-    const float o = blk[l][lc] * (1.f / NS_SCALE);
-    if (r.mom) {
-      float* p = reinterpret_cast<float*>(r.out) + at;
-      *p = *p * decay - f * o;
-    } else if (BF16) {
-      reinterpret_cast<unsigned short*>(r.out)[at] = g16_bf16(o);
-    } else {
-      reinterpret_cast<float*>(r.out)[at] = o;
-    }
+    put((int64_t)i * r.cols + j, blk[l][lc] * (1.f / NS_SCALE));
   }
 }
 
 struct NsPlan {
   std::vector<NsRec> recs;
   int64_t halves = 0, parts = 0;
-  bool alike = true;       // one length
+  bool alike = true;       // one length (of the matrices; vectors have no products)
   int blocks = 0, sym[3] = {0, 0, 0}, upd[3] = {0, 0, 0};        // tiles of 64, 128 and 256
 };
 
@@ -323,6 +357,7 @@ static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
   });
   auto pad = [](int64_t v) { return (int)((v + G16_PAD - 1) / G16_PAD * G16_PAD); };
   int64_t blocks = 0, sym[3] = {0, 0, 0}, upd[3] = {0, 0, 0};
+  int length = 0;
   for (int64_t k = 0; k < n; ++k) {
     const NsTensor& s = ts[order[k]];
     NsRec r = {};
@@ -330,7 +365,8 @@ static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
     r.rows = (int)s.rows; r.cols = (int)s.cols;
     r.m = std::min(r.rows, r.cols); r.n = std::max(r.rows, r.cols);
     r.mp = pad(r.m); r.np = pad(r.n);
-    const int64_t x = 2 * (int64_t)r.mp * r.np, a = 2 * (int64_t)r.mp * r.mp;
+    const bool vector = r.m == 1;                        // (no planes and no products)
+    const int64_t x = vector ? 0 : 2 * (int64_t)r.mp * r.np, a = vector ? 0 : 2 * (int64_t)r.mp * r.mp;
     r.x0 = out->halves; r.x1 = r.x0 + x; r.a = r.x1 + x; r.b = r.a + a;
     out->halves = r.b + a;
     const int64_t nb = (int64_t)(r.mp / NS_BLK) * (r.np / NS_BLK);
@@ -341,12 +377,13 @@ static int ns_plan(const NsTensor* ts, int64_t n, NsPlan* out) {
     out->parts += r.nparts;
     r.e0 = (int)blocks; blocks += nb;
     for (int k3 = 0; k3 < 3; ++k3) {
-      const int64_t tm = ceil_div(r.mp, 64 << k3), tn = ceil_div(r.np, 64 << k3);
+      const int64_t tm = vector ? 0 : ceil_div(r.mp, 64 << k3), tn = vector ? 0 : ceil_div(r.np, 64 << k3);
       r.s[k3] = (int)sym[k3]; r.u[k3] = (int)upd[k3];
       sym[k3] += tm * (tm + 1) / 2;
       upd[k3] += tm * tn;
     }
-    if (k && r.np != out->recs[0].np) out->alike = false;
+    if (!vector && length && r.np != length) out->alike = false;
+    if (!vector) length = r.np;
     if (blocks >= (1ll << 30) || sym[0] >= (1ll << 30) || upd[0] >= (1ll << 30)) return OFQ_EINVAL;
     out->recs.push_back(r);
   }
@@ -412,7 +449,7 @@ extern "C" int ofq_newton_schulz(const void* tensors, int64_t n, int bf16, int s
     auto grid = [](const int (&tiles)[3], int form) { return dim3((unsigned)tiles[form == G16_TINY ? 0 : form == G16_BIG ? 2 : 1]); };
     const dim3 ga = grid(p.sym, ca), gs = grid(p.sym, cs), gu = grid(p.upd, cu);
     const int ra = p.alike ? 32 : 4;
-    for (int k = 0; k < steps; ++k) {
+    for (int k = 0; k < (p.upd[0] ? steps : 0); ++k) {
 #define NS_SYM(CFG, SQ, GRID, RUN) hipLaunchKernelGGL((ns_sym_kernel<CFG, SQ>), GRID, dim3(g16_nt(CFG)), 0, st, recs, nn, fb, fc, k & 1, RUN, planes)
       if (ca == G16_BIG) NS_SYM(G16_BIG, false, ga, 32); else if (ca == G16_MID) NS_SYM(G16_MID, false, ga, 64);
       else if (ca == G16_DEEP) NS_SYM(G16_DEEP, false, ga, ra); else NS_SYM(G16_TINY, false, ga, ra);
@@ -426,8 +463,9 @@ extern "C" int ofq_newton_schulz(const void* tensors, int64_t n, int bf16, int s
       OFQ_LAUNCH_CHECK();
 #undef NS_UPD
     }
-    if (bf16) hipLaunchKernelGGL(ns_apply_kernel<true>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, hyper, gd, steps & 1, planes);
-    else hipLaunchKernelGGL(ns_apply_kernel<false>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, hyper, gd, steps & 1, planes);
+    const NsChain ch = {fa, fb, fc, eps, steps};
+    if (bf16) hipLaunchKernelGGL(ns_apply_kernel<true>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, ch, hyper, gd, parts, planes);
+    else hipLaunchKernelGGL(ns_apply_kernel<false>, dim3(p.blocks), dim3(256), 0, st, recs, nn, s, ch, hyper, gd, parts, planes);
     OFQ_LAUNCH_CHECK();
     return 0;
   } catch (...) { return OFQ_EINVAL; }
