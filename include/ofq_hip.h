@@ -562,7 +562,7 @@ int ofq_input_pipeline_u8(const uint8_t* in, float* out, int64_t B, int64_t C, i
  *  none is to come; the backward pass refuses another size than its own), ws: scratch; both 256-byte aligned device memory of the caller.
  *  bwd: grad = the incoming gradient (one float; reduction 0: [T]); dx [T][D], dw [V][D] in the tensors' type, db [V] in the
  *  bias's; any of them NULL.  The gradient of the logits exists for a piece of the vocabulary at a time.  reduction 0: the rows' gradients may
- *  be of any size next to each other (a row of dx is right to its own).
+ *  be of unlike size (a row of dx is right to its own, down to 1e-36 of the largest).
  *  T <= 2^24, V <= 2^24, D <= 2^20. */
 size_t ofq_linear_ce_kept_bytes(int64_t T, int64_t D, int64_t V, int bf16, int w_aligned, int backward);
 size_t ofq_linear_ce_fwd_ws_bytes(int64_t T, int64_t D, int64_t V, int bf16);
